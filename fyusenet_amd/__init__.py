@@ -12,3 +12,4 @@ from .builders import (ActType, ArgMaxLayerBuilder, ArithType, BlurKernelType, B
                        SingletonArithLayerBuilder, TransposeLayerBuilder, UpDownLayerBuilder)
 from .capi import FynException, ORDER_CHANNELWISE, ORDER_GPU_DEEP, ORDER_GPU_SHALLOW, STORAGE_F16, STORAGE_F32  # noqa: F401
 from .network import BufferManager, CompiledLayers, FramePool, Layer, LayerFactory, NeuralNetwork  # noqa: F401
+from .sequence import DeviceArray, SequenceCache, attention  # noqa: F401

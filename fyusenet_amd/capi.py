@@ -90,9 +90,36 @@ class CustomLayer(ctypes.Structure):
     _fields_ = [("user", ctypes.c_void_p), ("setup", CUSTOM_SETUP_FN), ("forward", CUSTOM_FORWARD_FN), ("cleanup", CUSTOM_CLEANUP_FN)]
 
 
+class Rows(ctypes.Structure):
+    """struct fyn_rows."""
+    _fields_ = [("data", ctypes.c_void_p), ("sequence_pitch", ctypes.c_int64), ("token_pitch", ctypes.c_int64), ("head_pitch", ctypes.c_int64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """struct fyn_attention_desc."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("storage", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("lengths", ctypes.c_void_p),
+                ("queries", Rows), ("keys", Rows), ("values", Rows), ("result", Rows)]
+
+
+class CacheDesc(ctypes.Structure):
+    """struct fyn_cache_desc."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("storage", ctypes.c_int32), ("layers", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("sequences", ctypes.c_int32), ("most_tokens", ctypes.c_int32)]
+
+
+class AttendDesc(ctypes.Structure):
+    """struct fyn_attend_desc."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("rows", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("queries", Rows), ("result", Rows)]
+
+
 # every symbol include/fynhip.h declares: name -> (restype, argtypes)
 _P = ctypes.c_void_p
 _F = ctypes.POINTER(ctypes.c_float)
+_I = ctypes.POINTER(ctypes.c_int32)
 SYMBOLS = {
     "fyn_last_error": (ctypes.c_char_p, []),
     "fyn_device_info": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]),
@@ -130,6 +157,21 @@ SYMBOLS = {
     "fyn_layer_kernel_info": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]),
     "fyn_host_acquire": (ctypes.c_int, [ctypes.c_size_t, ctypes.POINTER(_P)]),
     "fyn_host_release": (ctypes.c_int, [_P]),
+    "fyn_attention": (ctypes.c_int, [ctypes.POINTER(AttentionDesc), _P]),
+    "fyn_cache_create": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CacheDesc), ctypes.POINTER(_P)]),
+    "fyn_cache_destroy": (ctypes.c_int, [_P]),
+    "fyn_cache_extend": (ctypes.c_int, [_P, ctypes.c_int, _I, _I, _P]),
+    "fyn_cache_write": (ctypes.c_int, [_P, ctypes.c_int, ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.c_int, _P]),
+    "fyn_cache_attend": (ctypes.c_int, [_P, ctypes.c_int, ctypes.POINTER(AttendDesc), _P]),
+    "fyn_cache_read": (ctypes.c_int, [_P, ctypes.c_int, _I, ctypes.c_int, ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.c_int, _P]),
+    "fyn_cache_fork": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, _I, ctypes.c_int, _P]),
+    "fyn_cache_copy": (ctypes.c_int, [_P, ctypes.c_int, _I, _I, _P]),
+    "fyn_cache_truncate": (ctypes.c_int, [_P, ctypes.c_int, _I, _I, _P]),
+    "fyn_cache_free": (ctypes.c_int, [_P, ctypes.c_int, _I, _P]),
+    "fyn_cache_compact": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int), _P]),
+    "fyn_cache_lengths": (ctypes.c_int, [_P, ctypes.c_int, _I, _I]),
+    "fyn_cache_pages": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),
+    "fyn_cache_order": (ctypes.c_int, [_P, _P]),
     "fyn_net_device_allocations": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
 }
 

@@ -3,6 +3,7 @@
 #include <cstring>
 #include <string>
 
+#include "cache.h"
 #include "engine.h"
 
 struct fyn_net {
@@ -31,6 +32,21 @@ static thread_local std::string g_last_error;
 static fynhip::Net* N(fyn_net* n) {
     if (!n || !n->impl) fynhip::fail(FYN_ERR_INVALID, "null network handle");
     return n->impl;
+}
+
+static fynhip::Cache* C(fyn_cache* c) {
+    if (!c || !c->impl) fynhip::fail(FYN_ERR_INVALID, "null cache handle");
+    return c->impl.get();
+}
+template <class D>
+static const D& sized(const D* d, const char* name) {
+    if (!d) fynhip::fail(FYN_ERR_INVALID, "no %s given", name);
+    if (d->struct_size != sizeof(D)) fynhip::fail(FYN_ERR_INVALID, "%s size mismatch (%u, library expects %zu)", name, d->struct_size, sizeof(D));
+    return *d;
+}
+static const fyn_rows& given(const fyn_rows* r) {
+    if (!r) fynhip::fail(FYN_ERR_INVALID, "no keys or values given");
+    return *r;
 }
 
 extern "C" {
@@ -309,6 +325,101 @@ int fyn_layer_kernel_info(fyn_net* net, int layer, char* buf, size_t buflen) {
     if (!buf || buflen == 0) fynhip::fail(FYN_ERR_INVALID, "null buffer");
     std::string s = N(net)->layer(layer)->info();
     snprintf(buf, buflen, "%s", s.c_str());
+    FYN_API_END
+}
+
+// ---- sequences ----
+int fyn_attention(const fyn_attention_desc* desc, void* hip_stream) {
+    FYN_API_BEGIN
+    fynhip::attention(sized(desc, "fyn_attention_desc"), static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_create(int device, const fyn_cache_desc* desc, fyn_cache** out) {
+    FYN_API_BEGIN
+    if (!out) fynhip::fail(FYN_ERR_INVALID, "null output pointer");
+    std::unique_ptr<fyn_cache> c(new fyn_cache);
+    c->impl = std::make_shared<fynhip::Cache>(device, sized(desc, "fyn_cache_desc"));
+    *out = c.release();
+    FYN_API_END
+}
+
+int fyn_cache_destroy(fyn_cache* cache) {
+    FYN_API_BEGIN
+    delete cache;
+    FYN_API_END
+}
+
+int fyn_cache_extend(fyn_cache* cache, int n, const int32_t* sequences, const int32_t* tokens, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->extend(n, sequences, tokens, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_write(fyn_cache* cache, int layer, const fyn_rows* keys, const fyn_rows* values, int rows, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->write(layer, given(keys), given(values), rows, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_attend(fyn_cache* cache, int layer, const fyn_attend_desc* desc, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->attend(layer, sized(desc, "fyn_attend_desc"), static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_read(fyn_cache* cache, int n, const int32_t* sequences, int layer, const fyn_rows* keys, const fyn_rows* values, int rows, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->read(n, sequences, layer, given(keys), given(values), rows, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_fork(fyn_cache* cache, int source, int n, const int32_t* targets, int tokens, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->fork(source, n, targets, tokens, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_copy(fyn_cache* cache, int n, const int32_t* sources, const int32_t* targets, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->copy(n, sources, targets, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_truncate(fyn_cache* cache, int n, const int32_t* sequences, const int32_t* tokens, void* hip_stream) {
+    FYN_API_BEGIN
+    if (n > 0 && !tokens) fynhip::fail(FYN_ERR_INVALID, "cache: no numbers of tokens given");
+    C(cache)->truncate(n, sequences, tokens, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_free(fyn_cache* cache, int n, const int32_t* sequences, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->truncate(n, sequences, nullptr, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_compact(fyn_cache* cache, int* used, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->compact(used, static_cast<hipStream_t>(hip_stream));
+    FYN_API_END
+}
+
+int fyn_cache_lengths(fyn_cache* cache, int n, const int32_t* sequences, int32_t* tokens) {
+    FYN_API_BEGIN
+    C(cache)->lengths(n, sequences, tokens);
+    FYN_API_END
+}
+
+int fyn_cache_pages(fyn_cache* cache, int* used, int* free_pages) {
+    FYN_API_BEGIN
+    C(cache)->pages(used, free_pages);
+    FYN_API_END
+}
+
+int fyn_cache_order(fyn_cache* cache, void* hip_stream) {
+    FYN_API_BEGIN
+    C(cache)->order(static_cast<hipStream_t>(hip_stream));
     FYN_API_END
 }
 

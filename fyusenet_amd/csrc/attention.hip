@@ -1,0 +1,466 @@
+// Attention over a sequence's keys and values, dense or in the pages of a cache.
+//
+// For a query at position i of a sequence of n tokens the visible positions are
+//     j < n,  j <= i (causal),  |i - j| < window or j < sinks (window > 0)
+// and with s_j = scale <q, k_j> the result is  sum_j exp(s_j) v_j / sum_j exp(s_j)  over them, zero where there are none.
+//
+// One pass over the keys: a running maximum m and, relative to it, the running sum of the weights and of the weighted
+// values; where m grows both are multiplied with exp(m_old - m_new).  All of that is held in 32 bits.
+#include "sequence.h"
+
+#include <cstdio>
+#include <type_traits>
+
+namespace fynhip {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr float kNone = -__builtin_huge_valf();
+
+// The positions that one query sees: [lo, hi) and [0, first).
+struct Sight {
+    int lo, hi, first;
+    __device__ bool sees(int j) const { return (j >= lo && j < hi) || j < first; }
+};
+
+__device__ __forceinline__ Sight sight_of(int pos, int len, int causal, int window, int sinks) {
+    Sight s;
+    const int last = causal ? min(pos + 1, len) : len;
+    s.lo = 0; s.hi = last; s.first = 0;
+    if (window > 0) {
+        s.lo = max(0, pos - window + 1);
+        s.hi = (int)min((int64_t)last, (int64_t)pos + window);
+        s.first = min(sinks, last);
+    }
+    return s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Columns of queries against steps of keys, without shared memory on the way.
+//
+// A workgroup has sixteen columns: one token's heads of one key head (a group shares its keys), or sixteen tokens of one
+// head.  Its four waves take the steps of 16 or 32 keys in turn and join their sums at the end.  In a step
+//     S^T [keys x columns]  = K Q^T         K straight from memory as the matrix instruction's first operand
+//     O^T [dims x columns] += V^T P^T       V^T likewise, P^T is what S^T's registers hold already
+// The instruction multiplies with any order of its inner index, as long as both operands have the same one.  The lanes
+// l/16 = g hold rows 4g..4g+3 of S^T, so the inner index of the second product is ordered by them: a lane loads the
+// values of the keys 4g..4g+3 of each sixteen, a few neighbouring dims at a time, and P^T never leaves its registers.
+// A dim's keys are brought together by byte permutes of the lane's own registers (half a one for each value).
+//
+// Memory bound where a group's heads are the columns: every key and value is read once, in rows of 16 bytes a lane.
+// ---------------------------------------------------------------------------------------------------------------------
+template <class T, int DIMS>
+struct Shape {
+    static constexpr bool F16 = std::is_same<T, _Float16>::value;
+    static constexpr int VEC = 16 / sizeof(T);                    // elements of a lane's load of K
+    static constexpr int KLOADS = DIMS / (4 * VEC);               // ... for one key: 4 lanes side by side
+    static constexpr int TILES = (!F16 && DIMS > 128) ? 1 : 2;    // sixteens of keys in a step
+    static constexpr int STEP = 16 * TILES;
+    static constexpr int E = DIMS / 16 < VEC ? DIMS / 16 : VEC;   // dims that a lane loads of V at once
+    static constexpr int BLOCKS = (DIMS + 16 * E - 1) / (16 * E);
+    static constexpr int PITCH = BLOCKS * 16 * E + 4;             // of the joined sums in LDS (floats)
+};
+// (the classes of dims: DIMS = 32, 64, 96, 128, 256; E = 2, 4, 8 (6 would not be a power of two), 8, 8 of fp16 and
+// 2, 4, 4, 4, 4 of fp32)
+template <class T>
+struct Shape<T, 96> {
+    static constexpr bool F16 = std::is_same<T, _Float16>::value;
+    static constexpr int VEC = 16 / sizeof(T), KLOADS = 96 / (4 * VEC), TILES = 2, STEP = 32, E = F16 ? 8 : 4, BLOCKS = F16 ? 1 : 2, PITCH = 132;
+};
+
+template <class T, int N> struct Vec;
+template <> struct Vec<_Float16, 8> { typedef h8 type; };
+template <> struct Vec<_Float16, 4> { typedef h4 type; };
+template <> struct Vec<_Float16, 2> { typedef h2 type; };
+template <> struct Vec<float, 4> { typedef f4 type; };
+template <> struct Vec<float, 2> { typedef f2 type; };
+
+__device__ __forceinline__ bool finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
+__device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000) != 0x7f800000; }
+
+template <class T, int DIMS, bool PAGED, bool BY_TOKEN>
+__global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
+    typedef Shape<T, DIMS> S;
+    typedef typename Vec<T, S::VEC>::type KVec;
+    typedef typename Vec<T, S::E>::type VVec;
+    constexpr bool F16 = S::F16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+
+    // Which part of which columns.  Workgroups that read the same keys for different sequences (branches of one sequence
+    // share pages) or columns lie eight apart, which is on one XCD and its L2, one behind the other.
+    const int group = p.heads / p.kv_heads, across = BY_TOKEN ? p.heads : p.kv_heads;
+    const int columns = p.tiles * p.batch;
+    const int id = blockIdx.x, x = (id / (8 * columns)) * 8 + id % 8, col_tile = id / 8 % columns;
+    if (x >= across * p.parts) return;
+    const int part = x / across, who = x % across, b = col_tile / p.tiles, tile = col_tile % p.tiles;
+    const int kv_head = BY_TOKEN ? who / group : who;
+
+    int len, count, row0, seq = b;
+    if (PAGED) {
+        if (b >= p.words.first[p.words.sequences + 1]) return;
+        seq = p.words.batch[b];
+        len = p.words.len[seq];
+        row0 = p.words.first[b];
+        count = min(p.words.first[b + 1], p.tokens) - row0;
+    } else {
+        len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
+        count = p.tokens;   // (rows behind the length see nothing: zero)
+        row0 = 0;
+    }
+    const int pos0 = PAGED ? len - (p.words.first[b + 1] - row0) : 0;
+    const int token_tile = BY_TOKEN ? tile : tile / ((group + 15) / 16);
+    const int tok = BY_TOKEN ? token_tile * 16 + c : token_tile;
+    if ((BY_TOKEN ? token_tile * 16 : token_tile) >= count) return;
+    const int in_group = BY_TOKEN ? 0 : tile % ((group + 15) / 16) * 16 + c;
+    const int head = BY_TOKEN ? who : kv_head * group + in_group;
+    const bool valid = BY_TOKEN ? tok < count : in_group < group;
+    const bool inside = PAGED || pos0 + tok < len;   // (a padded row sees nothing)
+
+    // what the columns see, one by one and together
+    Sight mine = sight_of(pos0 + tok, len, p.causal, p.window, p.sinks);
+    if (!valid || !inside) mine.lo = mine.hi = mine.first = 0;
+    const int tok_a = BY_TOKEN ? token_tile * 16 : tok, tok_b = BY_TOKEN ? min(tok_a + 15, (PAGED ? count : min(count, len)) - 1) : tok;
+    Sight any = sight_of(pos0 + tok_a, len, p.causal, p.window, p.sinks), all = any;
+    if (tok_b < tok_a || (!PAGED && pos0 + tok_a >= len)) {
+        any.lo = any.hi = any.first = 0;
+        all = any;
+    } else if (BY_TOKEN) {
+        const Sight last = sight_of(pos0 + tok_b, len, p.causal, p.window, p.sinks);
+        any.hi = last.hi; any.first = last.first;
+        all.lo = last.lo;
+    }
+    const int a_steps = (any.first + S::STEP - 1) / S::STEP, b_first = max(any.lo / S::STEP, a_steps);
+    const int b_steps = max(0, (any.hi + S::STEP - 1) / S::STEP - b_first), steps = a_steps + b_steps;
+    // (equal parts for every row, so that those of long and short sequences take equally long)
+    const int chunk = max(p.chunk, (steps + p.parts - 1) / p.parts), begin = part * chunk, end = min(steps, begin + chunk);
+    if (begin > 0 && begin >= end) return;
+    const int most = max(any.hi, any.first);   // positions from here on are not read
+
+    // queries: operand of the first product
+    KVec q[S::KLOADS];
+    {
+        const T* src = reinterpret_cast<const T*>(p.q.p) + (PAGED ? 0 : b * p.q.seq) + (int64_t)(row0 + tok) * p.q.tok + (int64_t)head * p.q.head;
+#pragma unroll
+        for (int s = 0; s < S::KLOADS; s++) {
+            const int d = (s * 4 + g) * S::VEC;
+            q[s] = valid && d < p.dim ? *reinterpret_cast<const KVec*>(src + d) : KVec{};
+        }
+    }
+    f4 acc[S::BLOCKS][S::E];
+#pragma unroll
+    for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+        for (int n = 0; n < S::E; n++) acc[i][n] = f4{0, 0, 0, 0};
+    float m = kNone, l = 0;   // (l: of this lane's keys only)
+
+    const char *kbase, *vbase;
+    if (PAGED) {
+        kbase = p.pages.pool + kv_head * p.pages.head_bytes;
+        vbase = kbase + p.pages.values;
+    } else {
+        kbase = p.k.p + (b * p.k.seq + kv_head * p.k.head) * (int64_t)sizeof(T);
+        vbase = p.v.p + (b * p.v.seq + kv_head * p.v.head) * (int64_t)sizeof(T);
+    }
+    const int* table = PAGED ? p.words.table + (int64_t)seq * p.words.table_pitch : nullptr;
+
+    for (int st = begin + wave; st < end; st += 4) {
+        const int at = (st < a_steps ? st : b_first + st - a_steps) * S::STEP;
+        int page[4] = {0, 0, 0, 0};
+        if (PAGED) {
+            const int top = (most - 1) >> p.pages.shift;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i == 0 || (S::STEP >> p.pages.shift) > i) page[i] = table[min((at >> p.pages.shift) + i, top)];
+        }
+        auto row = [&](const char* base, int64_t tok_pitch, int off) -> const T* {   // of the key at + off; none behind the last visible one is read
+            const int j = min(at + off, most - 1);
+            if (PAGED) {
+                const int i = (j >> p.pages.shift) - (at >> p.pages.shift);
+                const int pg = i == 0 ? page[0] : i == 1 ? page[1] : i == 2 ? page[2] : page[3];
+                return reinterpret_cast<const T*>(base + pg * p.pages.page_bytes) + (j & ((1 << p.pages.shift) - 1)) * p.dim;
+            }
+            return reinterpret_cast<const T*>(base) + j * tok_pitch;
+        };
+        KVec k[S::TILES][S::KLOADS];
+        VVec v[S::TILES][4][S::BLOCKS];
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++) {
+            const T* src = row(kbase, p.k.tok, 16 * t + c);
+#pragma unroll
+            for (int s = 0; s < S::KLOADS; s++) {
+                const int d = (s * 4 + g) * S::VEC;
+                k[t][s] = d < p.dim ? *reinterpret_cast<const KVec*>(src + d) : KVec{};
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const T* src = row(vbase, p.v.tok, 16 * t + 4 * g + r);
+#pragma unroll
+                for (int i = 0; i < S::BLOCKS; i++) {
+                    const int d = (i * 16 + c) * S::E;
+                    v[t][r][i] = d < p.dim ? *reinterpret_cast<const VVec*>(src + d) : VVec{};
+                }
+            }
+        // scores
+        f4 sc[S::TILES];
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++) {
+            sc[t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < S::KLOADS; s++) {
+                if constexpr (F16) {
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], sc[t], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][s][e], q[s][e], sc[t], 0, 0, 0);
+                }
+            }
+            sc[t] *= p.scale_log2;
+        }
+        // Whether every column sees every key of the step; if not, what a column does not see weighs nothing, whatever
+        // the memory holds there.
+        const bool whole = (at >= all.lo && at + S::STEP <= all.hi) || at + S::STEP <= all.first;
+        bool fix = false;
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = at + 16 * t + 4 * g + r;
+                    if (!mine.sees(j)) sc[t][r] = kNone;
+                    const bool used = any.sees(j);
+#pragma unroll
+                    for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+                        for (int n = 0; n < S::E; n++) {
+                            if (!used) v[t][r][i][n] = 0;
+                            if (BY_TOKEN && !finite(v[t][r][i][n])) {   // a value that one column sees and another does not
+                                v[t][r][i][n] = 0;
+                                fix = true;
+                            }
+                        }
+                }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) top = fmaxf(top, sc[t][r]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m_new = fmaxf(m, top), base = m_new == kNone ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m - base);   // (m = none: 0)
+        m = m_new;
+        // Weights are kept 2^14 times as large: in 16 bits they then have their full precision down to 2^-28 of the
+        // largest, and what rounding takes from them is a second operand of the product.
+        f4 w[S::TILES];
+        float sum = 0;
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                w[t][r] = __builtin_amdgcn_exp2f(sc[t][r] - base + 14.f);
+                sum += w[t][r];
+            }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+            for (int n = 0; n < S::E; n++) acc[i][n] *= alpha;
+        if constexpr (F16) {
+            h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                hi[e] = (_Float16)w[e / 4][e % 4];
+                lo[e] = (_Float16)(w[e / 4][e % 4] - (float)hi[e]);
+            }
+#pragma unroll
+            for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+                for (int n = 0; n < S::E; n++) {
+                    h8 vt;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) vt[e] = v[e / 4][e % 4][i][n];
+                    acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, hi, acc[i][n], 0, 0, 0);
+                    acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, lo, acc[i][n], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+                        for (int n = 0; n < S::E; n++) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][r][i][n], w[t][r], acc[i][n], 0, 0, 0);
+        }
+        // Infinities and NaN among the values of such a step: only for the columns that see them.
+        if (BY_TOKEN && __any(fix)) {
+            for (int off = 0; off < S::STEP; off++) {
+                const int t = off / 16, owner = off % 16 / 4, r = off % 4;
+                float weight = 0;
+#pragma unroll
+                for (int tt = 0; tt < S::TILES; tt++)
+#pragma unroll
+                    for (int rr = 0; rr < 4; rr++)
+                        if (tt == t && rr == r) weight = w[tt][rr];
+                weight = __shfl(weight, owner * 16 + c);
+                const T* src = row(vbase, p.v.tok, off);
+#pragma unroll
+                for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+                    for (int n = 0; n < S::E; n++)
+#pragma unroll
+                        for (int rr = 0; rr < 4; rr++) {
+                            const int d = (i * 16 + 4 * g + rr) * S::E + n;
+                            if (d < p.dim && mine.sees(at + off)) {
+                                const T val = src[d];
+                                if (!finite(val)) acc[i][n][rr] += weight * (float)val;
+                            }
+                        }
+            }
+        }
+    }
+
+    // the four waves' sums: each has a maximum of its own
+    __shared__ __attribute__((aligned(16))) float sums[4][16][S::PITCH];
+    __shared__ float tops[4][16], totals[4][16];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+        tops[wave][c] = m;
+        totals[wave][c] = l;
+    }
+    // (sums[][column][dim]: register n of block i, row 4g+r is dim (16 i + 4g + r) E + n)
+#pragma unroll
+    for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int n = 0; n < S::E; n++) sums[wave][c][(i * 16 + 4 * g + r) * S::E + n] = acc[i][n][r];
+    __syncthreads();
+    // (sixteen threads for a column)
+    const int col = threadIdx.x >> 4, sub = threadIdx.x & 15;
+    const int o_tok = BY_TOKEN ? token_tile * 16 + col : token_tile;
+    const int o_in = BY_TOKEN ? 0 : in_group - c + col, o_head = BY_TOKEN ? who : kv_head * group + o_in;
+    if (BY_TOKEN ? o_tok >= count : o_in >= group) return;
+    float mm = kNone;
+    for (int w = 0; w < 4; w++) mm = fmaxf(mm, tops[w][col]);
+    const float base = mm == kNone ? 0.f : mm;
+    float f[4], total = 0;
+    for (int w = 0; w < 4; w++) {
+        f[w] = __builtin_amdgcn_exp2f(tops[w][col] - base);
+        total += totals[w][col] * f[w];
+    }
+    const bool only = steps <= chunk;   // the row has one part
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const bool zero = !PAGED && o_tok >= len;   // (a padded row: its column took part in steps that all others see whole)
+    const int64_t r_out = (int64_t)row0 + o_tok;
+    T* dst = reinterpret_cast<T*>(p.out.p) + (PAGED ? 0 : b * p.out.seq) + r_out * p.out.tok + (int64_t)o_head * p.out.head;
+    const int64_t cell = ((PAGED ? r_out : (int64_t)b * p.tokens + r_out) * p.heads + o_head) * p.parts + part;
+    for (int d = sub * 4; d < p.dim; d += 64) {
+        f4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) o += *reinterpret_cast<const f4*>(&sums[w][col][d]) * f[w];
+        if (only) {
+            typename Vec<T, 4>::type t;
+#pragma unroll
+            for (int e = 0; e < 4; e++) t[e] = zero ? (T)0 : (T)(o[e] * inv);
+            *reinterpret_cast<typename Vec<T, 4>::type*>(dst + d) = t;
+        } else {
+            *reinterpret_cast<f4*>(p.part_o + cell * p.dim + d) = o;
+        }
+    }
+    if (!only && sub == 0) {
+        p.part_ml[2 * cell] = mm;
+        p.part_ml[2 * cell + 1] = total;
+    }
+}
+
+// The parts of a row of a paged batch: one wave for a row and head.
+template <class T, int DIMS>
+__global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
+    typedef Shape<T, DIMS> S;
+    const int lane = threadIdx.x & 63;
+    const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int head = (int)(cell % p.heads), n = p.words.first[p.words.sequences + 1];
+    const int64_t row = cell / p.heads;
+    if (row >= p.tokens || n <= 0 || row >= p.words.first[n]) return;
+    int lo = 0, hi = n;   // the sequence whose rows this one is among
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.words.first[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    const int len = p.words.len[p.words.batch[lo]], pos = len - (p.words.first[lo + 1] - (int)row);
+    // the parts that attend_steps made
+    const Sight see = sight_of(pos, len, p.causal, p.window, p.sinks);
+    const int a_steps = (see.first + S::STEP - 1) / S::STEP, b_first = max(see.lo / S::STEP, a_steps);
+    const int steps = a_steps + max(0, (see.hi + S::STEP - 1) / S::STEP - b_first);
+    const int chunk = max(p.chunk, (steps + p.parts - 1) / p.parts);
+    if (steps <= chunk) return;
+    const int parts = (steps + chunk - 1) / chunk;
+    const float* ml = p.part_ml + 2 * cell * p.parts;
+    float m = kNone;
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[2 * i]);
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
+    const float base = m == kNone ? 0.f : m;
+    float total = 0;
+    f4 o = {0, 0, 0, 0};
+    const int d = lane * 4;
+    for (int i = 0; i < parts; i++) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * i] - base);
+        total += f * ml[2 * i + 1];
+        if (d < p.dim) o += *reinterpret_cast<const f4*>(p.part_o + (cell * p.parts + i) * p.dim + d) * f;
+    }
+    if (d >= p.dim) return;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    typename Vec<T, 4>::type t;
+#pragma unroll
+    for (int e = 0; e < 4; e++) t[e] = (T)(o[e] * inv);
+    *reinterpret_cast<typename Vec<T, 4>::type*>(reinterpret_cast<T*>(p.out.p) + row * p.out.tok + (int64_t)head * p.out.head + d) = t;
+}
+
+template <class T, int DIMS>
+static void launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
+    if (p.paged) {
+        if (p.by_token) hipLaunchKernelGGL((attend_steps<T, DIMS, true, true>), dim3(blocks), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((attend_steps<T, DIMS, true, false>), dim3(blocks), dim3(256), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((attend_steps<T, DIMS, false, true>), dim3(blocks), dim3(256), 0, s, p);
+    }
+    if (p.parts > 1) hipLaunchKernelGGL((join_parts<T, DIMS>), dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, s, p);
+}
+
+int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }
+
+int launch_attention(const AttnParams& p, hipStream_t s) {
+    const int64_t across = p.by_token ? p.heads : p.kv_heads;
+    const int64_t blocks = (across * p.parts + 7) / 8 * 8 * (int64_t)p.tiles * p.batch;
+    if (blocks <= 0) return 0;
+    if (blocks > 0x7fffffff) return -1;
+#define FYN_ATTN(T, D) launch_steps<T, D>(p, (unsigned)blocks, s)
+    if (p.f16) {
+        if (p.dim <= 32) FYN_ATTN(_Float16, 32);
+        else if (p.dim <= 64) FYN_ATTN(_Float16, 64);
+        else if (p.dim <= 96) FYN_ATTN(_Float16, 96);
+        else if (p.dim <= 128) FYN_ATTN(_Float16, 128);
+        else FYN_ATTN(_Float16, 256);
+    } else {
+        if (p.dim <= 32) FYN_ATTN(float, 32);
+        else if (p.dim <= 64) FYN_ATTN(float, 64);
+        else if (p.dim <= 96) FYN_ATTN(float, 96);
+        else if (p.dim <= 128) FYN_ATTN(float, 128);
+        else FYN_ATTN(float, 256);
+    }
+#undef FYN_ATTN
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace fynhip

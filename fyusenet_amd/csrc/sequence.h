@@ -1,0 +1,94 @@
+// Parameter blocks and host-side launchers of the kernels on sequences: attention (attention.hip) and the pages of a cache
+// of keys and values (cache_pages.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fynhip {
+
+constexpr int kMaxHeadDim = 256;
+
+// Rows of a tensor [sequence, token, head, dim], distances in elements; dim is dense.
+struct SeqRows {
+    char* p;
+    int64_t seq, tok, head;
+};
+
+// Where a cache keeps its int32 words on the device (page_book.h writes them): tokens of each sequence, the sequences of
+// the current batch, the rows at which their new tokens begin (one more than there are sequences), and the lists of pages.
+struct CacheWords {
+    const int* len;
+    const int* batch;
+    const int* first;
+    const int* table;
+    int table_pitch;   // entries per sequence
+    int sequences;     // entries of batch; `first` has one more, and the number of sequences in the batch stands behind it
+};
+
+// Pages: [page][layer][keys or values][kv head][token][dim].
+struct PageLayout {
+    char* pool;             // (with the offset of the layer)
+    int64_t page_bytes;     // all layers
+    int64_t values;         // bytes from a head's keys to its values
+    int64_t head_bytes;
+    int shift;              // log2 of the tokens of a page
+};
+
+struct AttnParams {
+    SeqRows q, k, v, out;   // (k, v: where nothing is paged)
+    PageLayout pages;
+    CacheWords words;
+    const int* lengths;     // nothing paged: tokens of each sequence, or null
+    int paged, f16;
+    int batch, tokens;      // nothing paged: rows of each sequence; paged: rows of q in all
+    int heads, kv_heads, dim;
+    int causal, window, sinks;
+    float scale_log2;       // softmax scale times log2(e)
+    // rows of one launch
+    int by_token;           // a workgroup's columns: 1 sixteen tokens of a head, 0 one token and up to sixteen heads of a group
+    int tiles;              // column tiles per sequence and (by_token) head or (else) key head
+    // the long axis in parts
+    int chunk;              // key steps of one part
+    int parts;              // most parts of a row
+    float* part_o;          // [row * heads + head][part][dim]
+    float* part_ml;         // ... [2]: maximum and sum
+};
+
+// 0, or -1 where the launch failed.
+int launch_attention(const AttnParams& p, hipStream_t s);
+int attention_step(int f16, int dim);   // keys of one step of the kernel (AttnParams::chunk counts them)
+
+constexpr int kUpdateWords = 896;
+struct CacheUpdate {        // (a kernel argument: at most 4 KB of them)
+    int n;
+    int w[kUpdateWords];    // {first word, number of words, words ...} ...
+};
+void launch_cache_update(int* words, const CacheUpdate& u, hipStream_t s);
+constexpr int kRowCopies = 896;
+struct RowCopies {
+    int n, words;
+    int to[kRowCopies];
+};
+void launch_row_copies(int* table, int pitch, int from, const RowCopies& r, hipStream_t s);
+constexpr int kPageCopies = 448;
+struct PageCopies {
+    int n;
+    int from[kPageCopies], to[kPageCopies];
+};
+void launch_page_copies(char* pool, int64_t page_bytes, const PageCopies& c, hipStream_t s);
+
+struct CacheRows {          // tokens between a cache and tensors
+    SeqRows k, v;
+    PageLayout pages;
+    CacheWords words;
+    int rows, kv_heads, dim, f16;
+};
+void launch_cache_write(const CacheRows& p, hipStream_t s);
+constexpr int kReadSequences = 400;
+struct CacheRead {
+    int n;
+    int sequence[kReadSequences], first[kReadSequences + 1];   // rows of the tensors, of this launch
+};
+void launch_cache_read(const CacheRows& p, const CacheRead& r, hipStream_t s);
+
+}  // namespace fynhip

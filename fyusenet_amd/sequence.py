@@ -1,0 +1,196 @@
+"""Attention over sequences, and the paged cache of their keys and values (the "sequences" part of include/fynhip.h).
+
+Tensors are device memory of the caller's: anything with data_ptr(), dtype, shape and stride() (torch tensors), anything
+with __cuda_array_interface__, a capi.TensorView as custom layers get them, or a DeviceArray.  `stream` is a hipStream_t as
+an integer (torch.cuda.current_stream().cuda_stream), 0 the default stream.  Calls return before the work is done.
+"""
+import ctypes
+
+import numpy as np
+
+from . import capi
+
+_SIZE = {capi.STORAGE_F16: 2, capi.STORAGE_F32: 4}
+
+
+class DeviceArray:
+    """Device memory: address, element type ("float16", "float32" or "int32"), shape, and distances in elements (dense if
+    not given)."""
+
+    __slots__ = ("ptr", "dtype", "shape", "strides")
+
+    def __init__(self, ptr, dtype, shape, strides=None):
+        self.ptr, self.dtype, self.shape = int(ptr), str(dtype), tuple(shape)
+        if strides is None:
+            strides, n = [], 1
+            for m in reversed(self.shape):
+                strides.insert(0, n)
+                n *= m
+        self.strides = tuple(strides)
+
+    @staticmethod
+    def of(x, name, heads=0):
+        """`x` as a DeviceArray; a TensorView [height, width, channels] becomes [height, width, heads, channels / heads]."""
+        if isinstance(x, DeviceArray):
+            return x
+        if hasattr(x, "data_ptr"):
+            if not getattr(x, "is_cuda", True):
+                raise capi.FynException(capi.ERR_INVALID, "%s: not device memory" % name)
+            return DeviceArray(x.data_ptr(), str(x.dtype).rpartition(".")[2], x.shape, x.stride())
+        if isinstance(x, capi.TensorView):
+            if x.channels % max(1, heads):
+                raise capi.FynException(capi.ERR_INVALID, "%s: %d channels are not %d heads" % (name, x.channels, heads))
+            wide, dim = x.width + 2 * x.padding, x.channels // max(1, heads)
+            typ = "float16" if x.storage == capi.STORAGE_F16 else "float32"
+            return DeviceArray((x.data or 0) + (x.padding * wide + x.padding) * x.channel_pitch * _SIZE[x.storage], typ,
+                               (x.height, x.width, heads, dim), (wide * x.channel_pitch, x.channel_pitch, dim, 1))
+        if hasattr(x, "__cuda_array_interface__"):
+            a = x.__cuda_array_interface__
+            dtype = np.dtype(a["typestr"])
+            strides = a.get("strides")
+            return DeviceArray(a["data"][0], dtype.name, a["shape"], strides and [s // dtype.itemsize for s in strides])
+        raise capi.FynException(capi.ERR_INVALID, "%s: not device memory" % name)
+
+
+_TYPES = {capi.STORAGE_F16: "float16", capi.STORAGE_F32: "float32"}
+
+
+def _rows(a, name, storage, shape, r):
+    """Fills the Rows `r` with tensor `a` of shape [.., token, head, dim]."""
+    if a.dtype != _TYPES[storage]:
+        raise capi.FynException(capi.ERR_INVALID, "%s: %s values, %s are expected" % (name, a.dtype, _TYPES[storage]))
+    if tuple(a.shape) != shape:
+        raise capi.FynException(capi.ERR_INVALID, "%s: shape %s, %s is expected" % (name, tuple(a.shape), shape))
+    st = a.strides
+    if st[-1] != 1 and shape[-1] > 1:
+        raise capi.FynException(capi.ERR_INVALID, "%s: the values of a head have to lie side by side" % name)
+    # (a distance that nothing is multiplied with may be anything)
+    r.data, r.head_pitch, r.token_pitch = a.ptr, st[-2] if shape[-2] > 1 else 0, st[-3] if shape[-3] > 1 else 0
+    r.sequence_pitch = st[0] if len(shape) == 4 and shape[0] > 1 else 0
+
+
+def attention(queries, keys, values, result, lengths=None, causal=True, window=0, sinks=0, scale=0.0, heads=0, kv_heads=0, stream=0):
+    """fyn_attention: queries and result [batch, tokens, heads, dim], keys and values [batch, tokens, kv_heads, dim].
+    lengths: int32 [batch] or None.  heads and kv_heads are asked for only where tensors are given as TensorViews, whose
+    rows are the sequences."""
+    q, k = DeviceArray.of(queries, "queries", heads), DeviceArray.of(keys, "keys", kv_heads or heads)
+    v, out = DeviceArray.of(values, "values", kv_heads or heads), DeviceArray.of(result, "result", heads)
+    if len(q.shape) != 4 or len(k.shape) != 4:
+        raise capi.FynException(capi.ERR_INVALID, "attention: tensors [batch, tokens, heads, dim] are expected")
+    d = capi.AttentionDesc()
+    d.struct_size = ctypes.sizeof(d)
+    d.storage = capi.STORAGE_F16 if q.dtype == "float16" else capi.STORAGE_F32
+    d.batch, d.tokens, d.heads, d.head_dim = q.shape
+    d.kv_heads = k.shape[2]
+    shape, kv_shape = tuple(q.shape), (q.shape[0], q.shape[1], k.shape[2], q.shape[3])
+    _rows(q, "queries", d.storage, shape, d.queries)
+    _rows(k, "keys", d.storage, kv_shape, d.keys)
+    _rows(v, "values", d.storage, kv_shape, d.values)
+    _rows(out, "result", d.storage, shape, d.result)
+    if lengths is not None:
+        n = DeviceArray.of(lengths, "lengths")
+        if n.dtype != "int32" or tuple(n.shape) != shape[:1] or (shape[0] > 1 and n.strides[0] != 1):
+            raise capi.FynException(capi.ERR_INVALID, "lengths: %d int32 values side by side are expected" % shape[0])
+        d.lengths = n.ptr
+    d.causal, d.window, d.sinks, d.scale = 1 if causal else 0, window, sinks, scale
+    capi.check(capi.lib().fyn_attention(ctypes.byref(d), stream))
+
+
+def _ints(v):
+    return (ctypes.c_int32 * len(v))(*v)
+
+
+class SequenceCache:
+    """fyn_cache: keys and values of `sequences` sequences in `pages` pages of `page_tokens` tokens, for `layers` attention
+    layers of `heads` heads that share `kv_heads` key heads of `head_dim` values.
+
+    A step: extend(sequences, tokens) names the sequences that get new tokens and how many; then, for each layer,
+    write(layer, keys, values) and attend(layer, queries, result) take these tokens' rows, sequence after sequence, as
+    [rows, heads, dim]."""
+
+    def __init__(self, storage, layers, heads, kv_heads, head_dim, page_tokens, pages, sequences, most_tokens=0, device=0):
+        self._h = ctypes.c_void_p()
+        d = capi.CacheDesc(ctypes.sizeof(capi.CacheDesc), storage, layers, heads, kv_heads, head_dim, page_tokens, pages, sequences, most_tokens)
+        capi.check(capi.lib().fyn_cache_create(device, ctypes.byref(d), ctypes.byref(self._h)))
+        self.storage, self.layers, self.heads, self.kv_heads, self.head_dim = storage, layers, heads, kv_heads, head_dim
+        self.page_tokens, self.sequences = page_tokens, sequences
+
+    def _same(self, a, b, what):
+        if len(a) != len(b):
+            raise capi.FynException(capi.ERR_INVALID, "%s: %d sequences and %d values" % (what, len(a), len(b)))
+
+    def extend(self, sequences, tokens, stream=0):
+        self._same(sequences, tokens, "extend")
+        capi.check(capi.lib().fyn_cache_extend(self._h, len(sequences), _ints(sequences), _ints(tokens), stream))
+
+    def _kv(self, keys, values):
+        k, v = DeviceArray.of(keys, "keys"), DeviceArray.of(values, "values")
+        shape = (k.shape[0] if len(k.shape) == 3 else 0, self.kv_heads, self.head_dim)
+        rk, rv = capi.Rows(), capi.Rows()
+        _rows(k, "keys", self.storage, shape, rk)
+        _rows(v, "values", self.storage, shape, rv)
+        return rk, rv, shape[0]
+
+    def write(self, layer, keys, values, stream=0):
+        rk, rv, rows = self._kv(keys, values)
+        capi.check(capi.lib().fyn_cache_write(self._h, layer, ctypes.byref(rk), ctypes.byref(rv), rows, stream))
+
+    def attend(self, layer, queries, result, window=0, sinks=0, scale=0.0, stream=0):
+        q, out = DeviceArray.of(queries, "queries"), DeviceArray.of(result, "result")
+        shape = (q.shape[0] if len(q.shape) == 3 else 0, self.heads, self.head_dim)
+        d = capi.AttendDesc()
+        d.struct_size, d.rows, d.window, d.sinks, d.scale = ctypes.sizeof(d), shape[0], window, sinks, scale
+        _rows(q, "queries", self.storage, shape, d.queries)
+        _rows(out, "result", self.storage, shape, d.result)
+        capi.check(capi.lib().fyn_cache_attend(self._h, layer, ctypes.byref(d), stream))
+
+    def read(self, sequences, layer, keys, values, stream=0):
+        """Keys and values of whole sequences into [tokens of all of them, kv_heads, dim]."""
+        rk, rv, rows = self._kv(keys, values)
+        capi.check(capi.lib().fyn_cache_read(self._h, len(sequences), _ints(sequences), layer, ctypes.byref(rk), ctypes.byref(rv), rows, stream))
+
+    def fork(self, source, targets, tokens=-1, stream=0):
+        capi.check(capi.lib().fyn_cache_fork(self._h, source, len(targets), _ints(targets), tokens, stream))
+
+    def copy(self, sources, targets, stream=0):
+        self._same(sources, targets, "copy")
+        capi.check(capi.lib().fyn_cache_copy(self._h, len(sources), _ints(sources), _ints(targets), stream))
+
+    def truncate(self, sequences, tokens, stream=0):
+        self._same(sequences, tokens, "truncate")
+        capi.check(capi.lib().fyn_cache_truncate(self._h, len(sequences), _ints(sequences), _ints(tokens), stream))
+
+    def free(self, sequences, stream=0):
+        capi.check(capi.lib().fyn_cache_free(self._h, len(sequences), _ints(sequences), stream))
+
+    def compact(self, stream=0):
+        """-> the number of used pages, which are the first ones now."""
+        used = ctypes.c_int(0)
+        capi.check(capi.lib().fyn_cache_compact(self._h, ctypes.byref(used), stream))
+        return used.value
+
+    def lengths(self, sequences):
+        got = (ctypes.c_int32 * len(sequences))()
+        capi.check(capi.lib().fyn_cache_lengths(self._h, len(sequences), _ints(sequences), got))
+        return list(got)
+
+    def pages(self):
+        """-> pages in use, pages that are free."""
+        used, left = ctypes.c_int(0), ctypes.c_int(0)
+        capi.check(capi.lib().fyn_cache_pages(self._h, ctypes.byref(used), ctypes.byref(left)))
+        return used.value, left.value
+
+    def order(self, stream):
+        """What this cache's calls have queued comes before what is queued on this stream from now on."""
+        capi.check(capi.lib().fyn_cache_order(self._h, stream))
+
+    def close(self):
+        if self._h:
+            capi.check(capi.lib().fyn_cache_destroy(self._h))
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

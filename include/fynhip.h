@@ -307,6 +307,91 @@ int fyn_net_device_allocations(fyn_net* net, size_t* calls, size_t* bytes);
 /* Text description of the kernel variant chosen for a layer (for profiles / reports). */
 int fyn_layer_kernel_info(fyn_net* net, int layer, char* buf, size_t buflen);
 
+/* ---- sequences --------------------------------------------------------------------------------------------------
+ * Attention over the tokens of sequences, and a cache of their keys and values in pages.  The reference has no layer that
+ * mixes distant positions; everything here is without a counterpart in it.
+ *
+ * The calls take device memory and enqueue on a stream of the caller's (a hipStream_t, NULL: the default stream of the
+ * device); they return before the work is done.  The device is the one that the memory (or the cache) is on, whichever is
+ * current.  Sums and weights are held in 32 bits whatever the storage.
+ *
+ * A token at position i of n sees position j where j < n, and, if causal, j <= i, and, with a window > 0, |i - j| < window
+ * or j < sinks (the first tokens, which stay visible).  A query that sees nothing gives zero.  What a token does not see
+ * has no influence, whatever the memory holds there (infinities and NaN included).  Query head h uses key head
+ * h / (heads / kv_heads). */
+
+/* Rows of a tensor: element (sequence, token, head, x) is at sequence*sequence_pitch + token*token_pitch + head*head_pitch + x,
+ * in elements of the storage type.  Address and pitches are multiples of 16 bytes.  The cache's calls take tokens of all
+ * sequences of a batch one behind the other and do not look at sequence_pitch. */
+typedef struct fyn_rows {
+    void* data;
+    int64_t sequence_pitch, token_pitch, head_pitch;
+} fyn_rows;
+
+/* Every token of a padded batch over its own sequence.  lengths: device memory, `batch` numbers of tokens (read when the
+ * work runs, and taken as within 0 and `tokens`), or NULL: all have `tokens`.  Rows of the result behind a sequence's length are zero.  head_dim: a
+ * multiple of 8 up to 256.  scale: of the scores, 0 is 1/sqrt(head_dim).  The result must not overlap the other tensors. */
+typedef struct fyn_attention_desc {
+    uint32_t struct_size;
+    int32_t storage; /* fyn_storage */
+    int32_t batch, tokens, heads, kv_heads, head_dim;
+    int32_t causal, window, sinks;
+    float scale;
+    const int32_t* lengths;
+    fyn_rows queries, keys, values, result;
+} fyn_attention_desc;
+int fyn_attention(const fyn_attention_desc* desc, void* hip_stream);
+
+/* A cache of keys and values for `layers` attention layers.  Its memory is `pages` pages of `page_tokens` tokens (a power
+ * of two from 8 to 1024), each with the keys and values of all layers; a sequence is a list of them.  Sequences are named by
+ * 0 .. sequences-1 and are empty at first.  most_tokens: the longest that a sequence may become, 0: all pages.
+ * Calls may come from any thread, one after the other; a stream other than the last call's waits for the work of that one.
+ * The batch: fyn_cache_extend names the sequences that get new tokens, and how many; fyn_cache_write and fyn_cache_attend
+ * then take these tokens' rows, sequence after sequence.  Cutting, emptying or replacing one of its sequences ends the batch.
+ * Under stream capture only fyn_cache_write and fyn_cache_attend may be called; a replay works on the batch as it is then,
+ * which must have as many sequences and new tokens of each as at capture, and the replaying stream has to be ordered
+ * behind other calls by the caller (fyn_cache_order).  Replays of one cache must not overlap. */
+typedef struct fyn_cache fyn_cache;
+typedef struct fyn_cache_desc {
+    uint32_t struct_size;
+    int32_t storage; /* fyn_storage */
+    int32_t layers, heads, kv_heads, head_dim;
+    int32_t page_tokens, pages, sequences, most_tokens;
+} fyn_cache_desc;
+int fyn_cache_create(int device, const fyn_cache_desc* desc, fyn_cache** out);
+/* Waits for the device.  A network that a cache is bound to keeps it until it is destroyed itself. */
+int fyn_cache_destroy(fyn_cache* cache);
+/* Room for tokens[i] more tokens (0 or more) of sequences[i]; they are the batch from now on.  FYN_ERR_STATE and nothing
+ * changed where there are too few pages.  A page that is not full and that another sequence has too is copied. */
+int fyn_cache_extend(fyn_cache* cache, int n, const int32_t* sequences, const int32_t* tokens, void* hip_stream);
+/* Keys and values of the batch's new tokens: `rows` rows of kv_heads x head_dim. */
+int fyn_cache_write(fyn_cache* cache, int layer, const fyn_rows* keys, const fyn_rows* values, int rows, void* hip_stream);
+/* Attention of the batch's new tokens, causal, over everything that the cache has of their sequences; `rows` rows of
+ * heads x head_dim.  Rows behind the last of them are left as they are. */
+typedef struct fyn_attend_desc {
+    uint32_t struct_size;
+    int32_t rows, window, sinks;
+    float scale;
+    fyn_rows queries, result;
+} fyn_attend_desc;
+int fyn_cache_attend(fyn_cache* cache, int layer, const fyn_attend_desc* desc, void* hip_stream);
+/* Keys and values of whole sequences, one behind the other: `rows` rows of kv_heads x head_dim in all. */
+int fyn_cache_read(fyn_cache* cache, int n, const int32_t* sequences, int layer, const fyn_rows* keys, const fyn_rows* values, int rows, void* hip_stream);
+/* Empty sequences become branches of `source`: its first `tokens` tokens (-1: all) in the same pages. */
+int fyn_cache_fork(fyn_cache* cache, int source, int n, const int32_t* targets, int tokens, void* hip_stream);
+/* Empty sequences become copies of others, in pages of their own. */
+int fyn_cache_copy(fyn_cache* cache, int n, const int32_t* sources, const int32_t* targets, void* hip_stream);
+/* Sequences are cut to their first tokens[i] tokens; pages that none has any more are free. */
+int fyn_cache_truncate(fyn_cache* cache, int n, const int32_t* sequences, const int32_t* tokens, void* hip_stream);
+/* Sequences are emptied. */
+int fyn_cache_free(fyn_cache* cache, int n, const int32_t* sequences, void* hip_stream);
+/* The used pages become the first ones of the memory; *used (may be NULL): how many they are. */
+int fyn_cache_compact(fyn_cache* cache, int* used, void* hip_stream);
+int fyn_cache_lengths(fyn_cache* cache, int n, const int32_t* sequences, int32_t* tokens);
+int fyn_cache_pages(fyn_cache* cache, int* used, int* free_pages);
+/* What this cache's calls have queued so far comes before what is queued on this stream from now on. */
+int fyn_cache_order(fyn_cache* cache, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
