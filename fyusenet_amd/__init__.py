@@ -6,7 +6,7 @@ LayerBuilder / LayerFactory / NeuralNetwork description surface.  There is no CP
 package without the built library raises ImportError at the first call.
 """
 from . import capi  # noqa: F401
-from .builders import (ActType, ArgMaxLayerBuilder, ArithType, BlurKernelType, BlurLayerBuilder, CastLayerBuilder,  # noqa: F401
+from .builders import (ActType, ArgMaxLayerBuilder, ArithType, AttentionLayerBuilder, BlurKernelType, BlurLayerBuilder, CastLayerBuilder,  # noqa: F401
                        CastTarget, ConcatLayerBuilder, ConvLayerBuilder, CustomLayerBuilder, GPULayerBuilder, ImgExtractLayerBuilder,
                        LayerBuilder, LayerFlags, LayerType, NormType, PoolLayerBuilder, ScaleLayerBuilder, ScalingType,
                        SingletonArithLayerBuilder, TransposeLayerBuilder, UpDownLayerBuilder)

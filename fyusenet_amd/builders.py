@@ -13,6 +13,7 @@ CastLayerBuilder    -> fyusenet/gpu/castlayerbuilder.h
 TransposeLayerBuilder -> fyusenet/gpu/transposelayerbuilder.h
 ImgExtractLayerBuilder -> fyusenet/gpu/imgextractlayerbuilder.h
 BlurLayerBuilder    -> fyusenet/gpu/blurlayerbuilder.h
+AttentionLayerBuilder is this package's own
 
 Method names keep the reference's spelling (inputPadding, prefixAct, ...) so that a network
 description reads like samples/samplenetworks/resnet50.cpp.  A builder only collects fields; the
@@ -117,7 +118,8 @@ class LayerType(enum.IntEnum):
     BATCHNORM = 30
     GEMM = 31
     CUSTOM = 32
-    LAST_SUPPORTED = 33
+    ATTENTION = 33   # (without a counterpart in the reference)
+    LAST_SUPPORTED = 34
     ILLEGAL = 1000
 
 
@@ -521,6 +523,47 @@ class BlurLayerBuilder(GPULayerBuilder):
     def _fill(self, d):
         d.kernel = self.kernel_
         d.blur_type = int(self.blurType_)
+
+
+class AttentionLayerBuilder(GPULayerBuilder):
+    """Attention between the positions of a map, or of each row of it (without a counterpart in the reference): ports 0, 1
+    and 2 are queries of heads * headDim channels, keys and values of kvHeads * headDim; the output is like the queries."""
+
+    def __init__(self, heads, kvHeads, headDim, name):
+        super().__init__(name)
+        self.type_ = LayerType.ATTENTION
+        self.heads_, self.kvHeads_, self.headDim_ = heads, kvHeads, headDim
+        self.outputChannels_ = heads * headDim
+        self.inputChannels_ = (heads + 2 * kvHeads) * headDim
+        self.causal_, self.window_, self.sinks_, self.scale_, self.rows_ = False, 0, 0, 0.0, False
+
+    def causal(self):
+        """A position sees no later ones."""
+        self.causal_ = True
+        return self
+
+    def window(self, size, sinks=0):
+        """A position sees those less than `size` away and the first `sinks`."""
+        self.window_, self.sinks_ = size, sinks
+        return self
+
+    def scoreScale(self, scale):
+        """Factor of the scores, 1 / sqrt(headDim) if not given."""
+        self.scale_ = scale
+        return self
+
+    def rowsAreSequences(self):
+        self.rows_ = True
+        return self
+
+    def _fill(self, d):
+        d.num_inputs = 3
+        for i, n in enumerate((self.heads_, self.kvHeads_, self.kvHeads_)):
+            d.inputs[i].channels, d.inputs[i].padding, d.inputs[i].flags = n * self.headDim_, self.inputPadding_, 0
+
+    def attention(self):
+        return capi.AttentionLayer(capi.ctypes.sizeof(capi.AttentionLayer), self.heads_, self.kvHeads_, int(self.causal_), self.window_, self.sinks_,
+                                   int(self.rows_), self.scale_)
 
 
 class CustomLayerBuilder(GPULayerBuilder):

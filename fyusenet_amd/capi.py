@@ -103,6 +103,12 @@ class AttentionDesc(ctypes.Structure):
                 ("queries", Rows), ("keys", Rows), ("values", Rows), ("result", Rows)]
 
 
+class AttentionLayer(ctypes.Structure):
+    """struct fyn_attention_layer."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("rows_are_sequences", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 class CacheDesc(ctypes.Structure):
     """struct fyn_cache_desc."""
     _fields_ = [("struct_size", ctypes.c_uint32), ("storage", ctypes.c_int32), ("layers", ctypes.c_int32), ("heads", ctypes.c_int32),
@@ -171,6 +177,8 @@ SYMBOLS = {
     "fyn_cache_compact": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int), _P]),
     "fyn_cache_lengths": (ctypes.c_int, [_P, ctypes.c_int, _I, _I]),
     "fyn_cache_pages": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),
+    "fyn_net_add_attention_layer": (ctypes.c_int, [_P, ctypes.POINTER(LayerDesc), ctypes.POINTER(AttentionLayer)]),
+    "fyn_layer_bind_cache": (ctypes.c_int, [_P, ctypes.c_int, _P, ctypes.c_int]),
     "fyn_cache_order": (ctypes.c_int, [_P, _P]),
     "fyn_net_device_allocations": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
 }

@@ -29,6 +29,15 @@ static thread_local std::string g_last_error;
     }                                                   \
     return FYN_OK;
 
+static fyn_layer_desc described(const fyn_layer_desc* desc) {
+    if (!desc) fynhip::fail(FYN_ERR_INVALID, "No builder supplied to layer factory line");
+    if (desc->struct_size != sizeof(fyn_layer_desc))
+        fynhip::fail(FYN_ERR_INVALID, "fyn_layer_desc size mismatch (%u, library expects %zu)", desc->struct_size, sizeof(fyn_layer_desc));
+    fyn_layer_desc d = *desc;
+    d.name[FYN_NAME_LEN - 1] = 0;
+    return d;
+}
+
 static fynhip::Net* N(fyn_net* n) {
     if (!n || !n->impl) fynhip::fail(FYN_ERR_INVALID, "null network handle");
     return n->impl;
@@ -83,23 +92,14 @@ int fyn_net_destroy(fyn_net* net) {
 
 int fyn_net_add_layer(fyn_net* net, const fyn_layer_desc* desc) {
     FYN_API_BEGIN
-    if (!desc) fynhip::fail(FYN_ERR_INVALID, "No builder supplied to layer factory line");
-    if (desc->struct_size != sizeof(fyn_layer_desc))
-        fynhip::fail(FYN_ERR_INVALID, "fyn_layer_desc size mismatch (%u, library expects %zu)", desc->struct_size, sizeof(fyn_layer_desc));
-    fyn_layer_desc d = *desc;
-    d.name[FYN_NAME_LEN - 1] = 0;
-    N(net)->add_layer(d);
+    N(net)->add_layer(described(desc));
     FYN_API_END
 }
 
 int fyn_net_add_custom_layer(fyn_net* net, const fyn_layer_desc* desc, const fyn_custom_layer* impl) {
     FYN_API_BEGIN
-    if (!desc || !impl) fynhip::fail(FYN_ERR_INVALID, "No builder supplied to layer factory line");
-    if (desc->struct_size != sizeof(fyn_layer_desc))
-        fynhip::fail(FYN_ERR_INVALID, "fyn_layer_desc size mismatch (%u, library expects %zu)", desc->struct_size, sizeof(fyn_layer_desc));
-    fyn_layer_desc d = *desc;
-    d.name[FYN_NAME_LEN - 1] = 0;
-    N(net)->add_custom_layer(d, *impl);
+    if (!impl) fynhip::fail(FYN_ERR_INVALID, "No builder supplied to layer factory line");
+    N(net)->add_custom_layer(described(desc), *impl);
     FYN_API_END
 }
 
@@ -414,6 +414,21 @@ int fyn_cache_lengths(fyn_cache* cache, int n, const int32_t* sequences, int32_t
 int fyn_cache_pages(fyn_cache* cache, int* used, int* free_pages) {
     FYN_API_BEGIN
     C(cache)->pages(used, free_pages);
+    FYN_API_END
+}
+
+int fyn_net_add_attention_layer(fyn_net* net, const fyn_layer_desc* desc, const fyn_attention_layer* attention) {
+    FYN_API_BEGIN
+    N(net)->add_attention_layer(described(desc), sized(attention, "fyn_attention_layer"));
+    FYN_API_END
+}
+
+int fyn_layer_bind_cache(fyn_net* net, int layer, fyn_cache* cache, int cache_layer) {
+    FYN_API_BEGIN
+    fynhip::Net* n = N(net);
+    n->finish();   // (a pass that runs has what it was given)
+    n->layer(layer)->bind_cache(cache ? C(cache)->shared_from_this() : nullptr, cache_layer);
+    n->weights_changed();
     FYN_API_END
 }
 

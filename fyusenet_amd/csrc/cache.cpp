@@ -47,13 +47,14 @@ static void check_storage(int storage) {
     if (storage != FYN_STORAGE_F32 && storage != FYN_STORAGE_F16) fail(FYN_ERR_INVALID, "unknown storage type %d", storage);
 }
 
-void attention(const fyn_attention_desc& a, hipStream_t s) {
+bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     check_storage(a.storage);
     check_heads(a.heads, a.kv_heads, a.head_dim);
     check_sight(a.window, a.sinks, a.scale);
     if (a.batch < 0 || a.tokens < 0 || (int64_t)a.batch * a.tokens > 0x7fffffff) fail(FYN_ERR_INVALID, "attention: %d sequences of %d tokens", a.batch, a.tokens);
-    if (a.batch == 0 || a.tokens == 0) return;
-    const int f16 = a.storage == FYN_STORAGE_F16, device = check_rows("queries", a.queries, f16);
+    if (a.batch == 0 || a.tokens == 0) return false;
+    const int f16 = a.storage == FYN_STORAGE_F16;
+    device = check_rows("queries", a.queries, f16);
     if (check_rows("keys", a.keys, f16) != device || check_rows("values", a.values, f16) != device || check_rows("result", a.result, f16) != device)
         fail(FYN_ERR_INVALID, "attention: the tensors are on different devices");
     if (a.lengths) {
@@ -63,8 +64,7 @@ void attention(const fyn_attention_desc& a, hipStream_t s) {
             fail(FYN_ERR_INVALID, "lengths: not memory of the tensors' device");
         }
     }
-    OnDevice on(device);
-    AttnParams p{};
+    p = AttnParams{};
     p.q = rows_of(a.queries); p.k = rows_of(a.keys); p.v = rows_of(a.values); p.out = rows_of(a.result);
     p.lengths = a.lengths;
     p.f16 = f16;
@@ -76,6 +76,14 @@ void attention(const fyn_attention_desc& a, hipStream_t s) {
     p.tiles = (a.tokens + 15) / 16;
     p.chunk = 0x7fffffff;
     p.parts = 1;
+    return true;
+}
+
+void attention(const fyn_attention_desc& a, hipStream_t s) {
+    AttnParams p;
+    int device;
+    if (!attention_params(a, p, device)) return;
+    OnDevice on(device);
     if (launch_attention(p, s) != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
 }
 
@@ -170,6 +178,12 @@ void Cache::settle(hipStream_t s) {
 void Cache::order(hipStream_t s) {
     std::lock_guard<std::mutex> lock(mu_);
     OnDevice on(device);
+    enter(s);
+}
+
+void Cache::expect(int rows, hipStream_t s) {
+    std::lock_guard<std::mutex> lock(mu_);
+    if (rows != book_.batch_rows()) fail(FYN_ERR_INVALID, "cache: the batch has %d new tokens, the layer %d positions", book_.batch_rows(), rows);
     enter(s);
 }
 

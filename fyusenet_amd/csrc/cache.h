@@ -9,7 +9,7 @@
 
 namespace fynhip {
 
-class Cache {
+class Cache : public std::enable_shared_from_this<Cache> {
   public:
     Cache(int device, const fyn_cache_desc& d);
     ~Cache();
@@ -23,10 +23,12 @@ class Cache {
     void compact(int* used, hipStream_t s);
     void lengths(int n, const int* seqs, int* tokens);
     void pages(int* used, int* free);
+    void expect(int rows, hipStream_t s);   // a pass over the batch follows on this stream, for so many new tokens
     void order(hipStream_t s);   // what has been queued on the stream that the cache was used on last comes before what follows on this one
 
     const int device;
     const fyn_cache_desc d;
+    void check_layer(int layer) const { (void)layout(layer); }
 
   private:
     std::mutex mu_;
@@ -52,6 +54,7 @@ class Cache {
 
 // Attention over dense tensors.
 void attention(const fyn_attention_desc& a, hipStream_t s);
+bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device);   // checked; false: nothing to do
 
 // The current device for the length of a call.
 class OnDevice {

@@ -342,6 +342,14 @@ void Net::add_custom_layer(const fyn_layer_desc& d, const fyn_custom_layer& impl
     layers[d.number] = std::move(l);
 }
 
+void Net::add_attention_layer(const fyn_layer_desc& d, const fyn_attention_layer& attention) {
+    if (is_setup) fail(FYN_ERR_STATE, "cannot add layers after setup");
+    if (d.number < 0) fail(FYN_ERR_INVALID, "Must identify each layer with a valid number (found %d in the builder)", d.number);
+    if (layers.count(d.number)) fail(FYN_ERR_DUPLICATE, "Trying to insert a layer on a position that is already taken (%d)", d.number);
+    std::unique_ptr<Layer> l(create_attention_layer(this, d, attention));
+    layers[d.number] = std::move(l);
+}
+
 void Net::connect(int out_layer, int in_layer, int port) {
     if (is_setup) fail(FYN_ERR_STATE, "cannot connect layers after setup");
     Layer* src = layer(out_layer);
@@ -601,6 +609,7 @@ void Net::collect_timings() {
 void Net::forward(uint64_t* seq_out) {
     if (!is_setup) fail(FYN_ERR_STATE, "forward() called on a network that was not set up");
     FYN_HIP(hipSetDevice(device));
+    for (Layer* l : with_cache) l->before_pass(stream);
     seq++;
     if (seq_out) *seq_out = seq;
     const bool plain = timings || !dump_dir.empty();

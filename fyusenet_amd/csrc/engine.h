@@ -61,6 +61,7 @@ struct DevBuffer {
 };
 
 class Net;
+class Cache;
 
 // The FYNHIP_* environment switches (tests, experiments, tuning cache), read once when a network is created: nothing on
 // a launch path, and nothing during a later setup or weight load, looks at the environment again.
@@ -101,6 +102,8 @@ class Layer {
     // a sigmoid or tanh layer: its arguments, for the layer in front that computes it as well (computed_by), else null
     virtual const FuncParams* pointwise() const { return nullptr; }
     virtual void computed_by(int) {}
+    virtual void bind_cache(std::shared_ptr<Cache>, int) { fail(FYN_ERR_INVALID, "layer %s (%d) is not an attention layer", d.name, d.number); }
+    virtual void before_pass(hipStream_t) {}   // (Net::with_cache) on the host, before the layers run or are replayed
     Act act() const;
     const Tensor& tin(int port) const;
     const Tensor& tout() const;
@@ -118,6 +121,7 @@ class Net {
     ~Net();
     void add_layer(const fyn_layer_desc& d);
     void add_custom_layer(const fyn_layer_desc& d, const fyn_custom_layer& impl);
+    void add_attention_layer(const fyn_layer_desc& d, const fyn_attention_layer& attention);
     void connect(int out_layer, int in_layer, int port);
     void setup();
     void forward(uint64_t* seq);
@@ -161,6 +165,7 @@ class Net {
     std::vector<Tensor> tensors;
     std::vector<DevBuffer> buffers;
     uint64_t seq = 0;
+    std::vector<Layer*> with_cache;   // attention layers that work on a cache
 
     // Whether a tensor's buffer is the tensor's alone from layer `from` through layer `to`: no other tensor in it is
     // written by the launch of one of them, nor read by it.  Asked before a launch is made to write the tensor earlier
@@ -267,6 +272,7 @@ void fuse_depthwise_layers(Net* net);   // after every layer's setup(): depthwis
 void fuse_function_layers(Net* net);   // after every layer's setup(): sigmoid / tanh layers that the row-rolling convolution in front of them can apply to what it stores
 void fuse_concat_layers(Net* net);   // after every layer's setup(): bilinear scale layers in front of concatenations and batch-norm layers behind them
 void fuse_argmax_layers(Net* net);   // after every layer's setup(): arg-max layers that the streaming 1x1 convolution in front of them can compute
+Layer* create_attention_layer(Net* net, const fyn_layer_desc& d, const fyn_attention_layer& attention);
 Layer* create_custom_layer(Net* net, const fyn_layer_desc& d, const fyn_custom_layer& impl);
 
 }  // namespace fynhip

@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "engine.h"
+#include "cache.h"
 #include "conv_plan.h"
 #include "layer_classes.h"
 
@@ -639,6 +640,91 @@ class ArgMaxLayer : public Layer {
     int fused_into = -1;
 };
 
+// Attention between the positions of a map (or of each of its rows), or of them as new tokens over a cache.
+class AttentionLayer : public Layer {
+  public:
+    AttentionLayer(Net* n, const fyn_layer_desc& d_, const fyn_attention_layer& a_) : Layer(n, d_), at(a_) {
+        if (d.flags & ~FYN_FLAG_DEEP) fail(FYN_ERR_UNSUPPORTED, "attention layer %s: activations, norms and residual inputs are not supported", d.name);
+        if (d.num_inputs != 3) fail(FYN_ERR_INVALID, "attention layer %s takes queries, keys and values, not %d inputs", d.name, d.num_inputs);
+        if (at.heads < 1 || d.out_channels % at.heads) fail(FYN_ERR_INVALID, "attention layer %s: %d channels are not %d heads", d.name, d.out_channels, at.heads);
+        dim = d.out_channels / at.heads;
+        if (d.inputs[0].channels != d.out_channels || d.inputs[1].channels != (int64_t)at.kv_heads * dim || d.inputs[2].channels != (int64_t)at.kv_heads * dim)
+            fail(FYN_ERR_INVALID, "attention layer %s: inputs of %d, %d and %d channels for %d heads of %d values and %d key heads", d.name, d.inputs[0].channels,
+                 d.inputs[1].channels, d.inputs[2].channels, at.heads, dim, at.kv_heads);
+        for (int i = 0; i < 3; i++)
+            if (d.inputs[i].padding < 0) fail(FYN_ERR_INVALID, "layer %s: negative padding", d.name);
+        if (!at.rows_are_sequences && padded()) fail(FYN_ERR_UNSUPPORTED, "attention layer %s: padding is supported where rows are sequences", d.name);
+        if ((int64_t)d.height * d.width > 0x7fffffff) fail(FYN_ERR_INVALID, "attention layer %s: %dx%d positions", d.name, d.width, d.height);
+        oc = d.out_channels;
+        oh = d.height;
+        ow = d.width;
+        fyn_attention_desc a = desc();   // (what a call would refuse)
+        a.batch = 0;
+        AttnParams none;
+        int dev;
+        attention_params(a, none, dev);
+    }
+    int num_ports() const override { return 3; }
+    void port_shape(int port, int& c, int& h, int& w, int& pad) const override {
+        c = d.inputs[port].channels; h = d.height; w = d.width; pad = d.inputs[port].padding;
+    }
+    void setup() override {
+        fyn_attention_desc a = desc();
+        a.queries = rows(tin(0).v); a.keys = rows(tin(1).v); a.values = rows(tin(2).v); a.result = rows(tout().v);
+        int dev;
+        attention_params(a, p, dev);
+    }
+    void bind_cache(std::shared_ptr<Cache> c, int layer) override {
+        if (c) {
+            c->check_layer(layer);
+            if (!at.causal) fail(FYN_ERR_INVALID, "layer %s: a cache is for causal attention", d.name);
+            if (padded()) fail(FYN_ERR_UNSUPPORTED, "layer %s: a cache takes tensors without padding", d.name);
+            if (c->device != net->device || c->d.storage != net->storage || c->d.heads != at.heads || c->d.kv_heads != at.kv_heads || c->d.head_dim != dim)
+                fail(FYN_ERR_INVALID, "layer %s and the cache differ in device, storage, heads, key heads or values per head", d.name);
+        }
+        cache = std::move(c);
+        cache_layer = layer;
+        auto& w = net->with_cache;
+        w.erase(std::remove(w.begin(), w.end(), this), w.end());
+        if (cache) w.push_back(this);
+    }
+    void before_pass(hipStream_t s) override { cache->expect(oh * ow, s); }
+    void forward(hipStream_t s) override {
+        if (!cache) {
+            if (launch_attention(p, s) != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
+            return;
+        }
+        fyn_attend_desc a{};
+        a.rows = oh * ow;
+        a.window = at.window; a.sinks = at.sinks; a.scale = at.scale;
+        a.queries = rows(tin(0).v); a.result = rows(tout().v);
+        cache->write(cache_layer, rows(tin(1).v), rows(tin(2).v), a.rows, s);
+        cache->attend(cache_layer, a, s);
+    }
+    std::string info() const override { return cache ? "attention over a cache" : "attention"; }
+
+  private:
+    bool padded() const { return d.inputs[0].padding || d.inputs[1].padding || d.inputs[2].padding || d.output_padding; }
+    fyn_attention_desc desc() const {
+        fyn_attention_desc a{};
+        a.storage = net->storage;
+        a.batch = at.rows_are_sequences ? d.height : 1;
+        a.tokens = at.rows_are_sequences ? d.width : d.height * d.width;
+        a.heads = at.heads; a.kv_heads = at.kv_heads; a.head_dim = dim;
+        a.causal = at.causal; a.window = at.window; a.sinks = at.sinks; a.scale = at.scale;
+        return a;
+    }
+    fyn_rows rows(const TView& v) const {
+        const int64_t row = (int64_t)v.wp() * v.cp;
+        return fyn_rows{static_cast<char*>(v.ptr) + (v.pad * row + (int64_t)v.pad * v.cp) * (v.f16 ? 2 : 4), row, v.cp, dim};
+    }
+    const fyn_attention_layer at;
+    int dim = 0;
+    AttnParams p{};
+    std::shared_ptr<Cache> cache;
+    int cache_layer = 0;
+};
+
 class UploadLayer : public Layer {
   public:
     UploadLayer(Net* n, const fyn_layer_desc& d_) : Layer(n, d_) {
@@ -722,13 +808,25 @@ Layer* create_custom_layer(Net* net, const fyn_layer_desc& d, const fyn_custom_l
     return l;
 }
 
-Layer* create_layer(Net* net, const fyn_layer_desc& d) {
+static void check_shape(const fyn_layer_desc& d) {
     if (d.width <= 0 || d.height <= 0 || d.width > 65535 || d.height > 65535)
         fail(FYN_ERR_INVALID, "layer %s: invalid spatial size %dx%d", d.name, d.width, d.height);
     if (d.in_channels <= 0 || d.in_channels > 32767 || d.out_channels < 0 || d.out_channels > 32767)
         fail(FYN_ERR_INVALID, "layer %s: invalid channel counts %d -> %d", d.name, d.in_channels, d.out_channels);
     if (d.input_padding < 0 || d.output_padding < 0 || d.residual_padding < 0)
         fail(FYN_ERR_INVALID, "layer %s: negative padding", d.name);
+}
+
+Layer* create_attention_layer(Net* net, const fyn_layer_desc& d, const fyn_attention_layer& attention) {
+    if (d.type != FYN_LAYER_ATTENTION) fail(FYN_ERR_INVALID, "layer %s: an attention layer needs type FYN_LAYER_ATTENTION", d.name);
+    check_shape(d);
+    Layer* l = new AttentionLayer(net, d, attention);
+    l->in.assign(l->num_ports(), -1);
+    return l;
+}
+
+Layer* create_layer(Net* net, const fyn_layer_desc& d) {
+    check_shape(d);
     Layer* l = nullptr;
     switch (d.type) {
         case FYN_LAYER_CONVOLUTION2D: {
@@ -777,6 +875,7 @@ Layer* create_layer(Net* net, const fyn_layer_desc& d) {
             l = new ConvLayer(net, d);
             break;
         case FYN_LAYER_CUSTOM: fail(FYN_ERR_INVALID, "layer %s: custom layers are added with fyn_net_add_custom_layer", d.name);
+        case FYN_LAYER_ATTENTION: fail(FYN_ERR_INVALID, "layer %s: attention layers are added with fyn_net_add_attention_layer", d.name);
         case FYN_LAYER_UPLOAD: l = new UploadLayer(net, d); break;
         case FYN_LAYER_DOWNLOAD: l = new DownloadLayer(net, d); break;
         default: fail(FYN_ERR_UNSUPPORTED, "Unsupported layer type %d", d.type);

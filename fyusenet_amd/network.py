@@ -81,6 +81,10 @@ class Layer:
         capi.check(capi.lib().fyn_layer_kernel_info(self._net._h, self.number, buf, len(buf)))
         return buf.value.decode()
 
+    def bindCache(self, cache, cacheLayer=0):
+        """fyn_layer_bind_cache: an attention layer works on a SequenceCache from now on (None: no longer)."""
+        capi.check(capi.lib().fyn_layer_bind_cache(self._net._h, self.number, cache._h if cache is not None else None, cacheLayer))
+
     def timeKernel(self, iters):
         ms = ctypes.c_float(0)
         capi.check(capi.lib().fyn_layer_time(self._net._h, self.number, iters, ctypes.byref(ms)))
@@ -145,6 +149,10 @@ class LayerFactory:
             d = b.desc()
             if int(b.type_) == int(LayerType.CUSTOM):
                 self._add_custom(b, d)
+            elif int(b.type_) == int(LayerType.ATTENTION):
+                if not hasattr(b, "attention"):
+                    raise capi.FynException(capi.ERR_INVALID, "layer %s: an ATTENTION layer needs an AttentionLayerBuilder" % b.name_)
+                capi.check(capi.lib().fyn_net_add_attention_layer(self._net._h, ctypes.byref(d), ctypes.byref(b.attention())))
             else:
                 capi.check(capi.lib().fyn_net_add_layer(self._net._h, ctypes.byref(d)))
             layers._add(Layer(self._net, b))

@@ -68,7 +68,8 @@ enum fyn_layer_type {
     FYN_LAYER_UPLOAD = 27,
     FYN_LAYER_BATCHNORM = 30,
     FYN_LAYER_GEMM = 31,
-    FYN_LAYER_CUSTOM = 32 /* only through fyn_net_add_custom_layer */
+    FYN_LAYER_CUSTOM = 32, /* only through fyn_net_add_custom_layer */
+    FYN_LAYER_ATTENTION = 33 /* only through fyn_net_add_attention_layer */
 };
 
 /* LayerFlags bits (fyusenet/base/layerflags.h:33-50), as LayerBuilderTempl::getFlags() composes them
@@ -389,6 +390,21 @@ int fyn_cache_free(fyn_cache* cache, int n, const int32_t* sequences, void* hip_
 int fyn_cache_compact(fyn_cache* cache, int* used, void* hip_stream);
 int fyn_cache_lengths(fyn_cache* cache, int n, const int32_t* sequences, int32_t* tokens);
 int fyn_cache_pages(fyn_cache* cache, int* used, int* free_pages);
+/* Attention between the positions of a map as a layer of a network.  desc->type must be FYN_LAYER_ATTENTION.  Input ports:
+ * desc->num_inputs = 3 in desc->inputs[], queries of out_channels = heads * head_dim channels, keys and values of kv_heads *
+ * head_dim.  The positions of the whole map are one sequence, row by row, or, with rows_are_sequences, each row is one; padding is
+ * supported where rows are sequences.  The output is like the queries.  Both structs are copied. */
+typedef struct fyn_attention_layer {
+    uint32_t struct_size;
+    int32_t heads, kv_heads, causal, window, sinks, rows_are_sequences;
+    float scale;
+} fyn_attention_layer;
+int fyn_net_add_attention_layer(fyn_net* net, const fyn_layer_desc* desc, const fyn_attention_layer* attention);
+/* An attention layer of a network (causal, with the cache's storage, device, heads, key heads and values per head) works on
+ * the cache from now on: its positions, row by row, are the new tokens of the batch, whose keys and values the layer writes
+ * (as the cache's layer `cache_layer`) before it attends to the cache.  fyn_cache_extend comes before each pass;
+ * a pass is refused where the batch has not as many new tokens as the layer has positions.  The ports have no padding.  cache NULL: the layer is as described again. */
+int fyn_layer_bind_cache(fyn_net* net, int layer, fyn_cache* cache, int cache_layer);
 /* What this cache's calls have queued so far comes before what is queued on this stream from now on. */
 int fyn_cache_order(fyn_cache* cache, void* hip_stream);
 

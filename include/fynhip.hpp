@@ -77,7 +77,7 @@ inline void check(int status) {
 enum class LayerType : int {
     ADD = 1, SUB, ARGMAX, CAST, CONCAT, CONVOLUTION2D, FRACCONVOLUTION2D, TRANSCONVOLUTION2D, AVGPOOL2D, MAXPOOL2D,
     PADDING2D, SCALE2D, SINGLETON_ARITH, RELU, CLIP, TANH, SIGMOID, REDUCE, TRANSPOSE, IMGEXTRACT, BLUR2D, NONMAX2D,
-    RGB2BGR, DEEP2SHALLOW, SHALLOW2DEEP, DOWNLOAD, UPLOAD, RESIDUAL, OESCONV, BATCHNORM, GEMM, CUSTOM, LAST_SUPPORTED,
+    RGB2BGR, DEEP2SHALLOW, SHALLOW2DEEP, DOWNLOAD, UPLOAD, RESIDUAL, OESCONV, BATCHNORM, GEMM, CUSTOM, ATTENTION, LAST_SUPPORTED,
     ILLEGAL = 1000
 };
 enum class ActType : int { NONE = 0, RELU, LEAKY_RELU, CLIP, SIGMOID, TANH };
@@ -402,6 +402,37 @@ struct ImgExtractLayerBuilder : GPULayerBuilderTempl<ImgExtractLayerBuilder> {
     void fill(fyn_layer_desc& d) const override { d.window = window_; }
 };
 
+/* Attention between the positions of a map or of each of its rows (no counterpart in the reference): ports 0, 1 and 2 are
+ * queries of heads * headDim channels, keys and values of kvHeads * headDim. */
+struct AttentionLayerBuilder : GPULayerBuilderTempl<AttentionLayerBuilder> {
+    AttentionLayerBuilder(int heads, int kvHeads, int headDim, const std::string& name)
+        : GPULayerBuilderTempl<AttentionLayerBuilder>(name), heads_(heads), kvHeads_(kvHeads), headDim_(headDim) {
+        type_ = LayerType::ATTENTION;
+        outputChannels_ = heads * headDim;
+        inputChannels_ = (heads + 2 * kvHeads) * headDim;
+    }
+    AttentionLayerBuilder& causal() { causal_ = true; return *this; }
+    AttentionLayerBuilder& window(int size, int sinks = 0) { window_ = size; sinks_ = sinks; return *this; }
+    AttentionLayerBuilder& scoreScale(float scale) { scale_ = scale; return *this; }
+    AttentionLayerBuilder& rowsAreSequences() { rows_ = true; return *this; }
+    fyn_attention_layer attention() const {
+        return fyn_attention_layer{sizeof(fyn_attention_layer), heads_, kvHeads_, causal_, window_, sinks_, rows_, scale_};
+    }
+    int heads_, kvHeads_, headDim_;
+    bool causal_ = false, rows_ = false;
+    int window_ = 0, sinks_ = 0;
+    float scale_ = 0.f;
+
+  protected:
+    void fill(fyn_layer_desc& d) const override {
+        d.num_inputs = 3;
+        for (int i = 0; i < 3; i++) {
+            d.inputs[i].channels = (i ? kvHeads_ : heads_) * headDim_;
+            d.inputs[i].padding = inputPadding_;
+        }
+    }
+};
+
 struct BlurLayerBuilder : GPULayerBuilderTempl<BlurLayerBuilder> {
     explicit BlurLayerBuilder(const std::string& name) : GPULayerBuilderTempl<BlurLayerBuilder>(name) { type_ = LayerType::BLUR2D; }
     BlurLayerBuilder& kernel(short sz) { kernel_ = sz; return *this; }
@@ -485,6 +516,8 @@ class LayerBase {
     void setInput(const float* data, int port = 0, int order = FYN_ORDER_CHANNELWISE) {
         detail::check(fyn_net_set_input(net_, number_, port, data, order));
     }
+    /* An attention layer works on the cache from now on (null: no longer), as fyn_layer_bind_cache. */
+    void bindCache(fyn_cache* cache, int cacheLayer = 0) { detail::check(fyn_layer_bind_cache(net_, number_, cache, cacheLayer)); }
     size_t weightFloats() const {
         size_t n = 0;
         detail::check(fyn_layer_weight_floats(net_, number_, &n));
@@ -583,6 +616,7 @@ class LayerFactory {
             const LayerBuilderData& b = *kv.second;
             const fyn_layer_desc d = b.desc();
             if (b.type_ == LayerType::CUSTOM) addCustom(b, d);
+            else if (b.type_ == LayerType::ATTENTION) addAttention(b, d);
             else detail::check(fyn_net_add_layer(net_, &d));
             switch (b.type_) {
                 case LayerType::CONVOLUTION2D: case LayerType::FRACCONVOLUTION2D: case LayerType::TRANSCONVOLUTION2D: case LayerType::GEMM:
@@ -599,6 +633,12 @@ class LayerFactory {
     }
 
   private:
+    void addAttention(const LayerBuilderData& b, const fyn_layer_desc& d) {
+        const auto* ab = dynamic_cast<const gpu::AttentionLayerBuilder*>(&b);
+        if (!ab) detail::raise(FYN_ERR_INVALID, "layer %s: an ATTENTION layer needs an AttentionLayerBuilder", b.name_.c_str());
+        const fyn_attention_layer a = ab->attention();
+        detail::check(fyn_net_add_attention_layer(net_, &d, &a));
+    }
     void addCustom(const LayerBuilderData& b, const fyn_layer_desc& d) {
         // gpu/gpulayerfactory.cpp:586-589: the builder's callback creates the layer
         const auto* cb = dynamic_cast<const gpu::CustomLayerBuilder*>(&b);
