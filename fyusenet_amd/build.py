@@ -27,6 +27,7 @@ def build(verbose=True, jobs=8):
     # these once per storage type (fp32 tensors with the host entry points, fp16 tensors)
     for name in ("conv_p16", "conv_a16"):
         units += [(name + ".hip", name + ".f32.o", ["-DFYN_P16_HALF=0"]), (name + ".hip", name + ".f16.o", ["-DFYN_P16_HALF=1"])]
+    units += [("attention_tiles.hip", "attention_tiles.%s.o" % t, ["-DFYN_ATTN_HALF=%d" % h]) for t, h in (("f32", 0), ("f16", 1))]
     units += [(src, src + ".o", []) for src in SOURCES]
     for src, objname, defs in units:
         obj = os.path.join(objdir, objname)

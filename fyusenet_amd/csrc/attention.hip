@@ -6,38 +6,9 @@
 //
 // One pass over the keys: a running maximum m and, relative to it, the running sum of the weights and of the weighted
 // values; where m grows both are multiplied with exp(m_old - m_new).  All of that is held in 32 bits.
-#include "sequence.h"
-
-#include <cstdio>
-#include <type_traits>
+#include "attention_common.h"
 
 namespace fynhip {
-
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-
-constexpr float kNone = -__builtin_huge_valf();
-
-// The positions that one query sees: [lo, hi) and [0, first).
-struct Sight {
-    int lo, hi, first;
-    __device__ bool sees(int j) const { return (j >= lo && j < hi) || j < first; }
-};
-
-__device__ __forceinline__ Sight sight_of(int pos, int len, int causal, int window, int sinks) {
-    Sight s;
-    const int last = causal ? min(pos + 1, len) : len;
-    s.lo = 0; s.hi = last; s.first = 0;
-    if (window > 0) {
-        s.lo = max(0, pos - window + 1);
-        s.hi = (int)min((int64_t)last, (int64_t)pos + window);
-        s.first = min(sinks, last);
-    }
-    return s;
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Columns of queries against steps of keys, without shared memory on the way.
@@ -72,16 +43,6 @@ struct Shape<T, 96> {
     static constexpr int VEC = 16 / sizeof(T), KLOADS = 96 / (4 * VEC), TILES = 2, STEP = 32, E = F16 ? 8 : 4, BLOCKS = F16 ? 1 : 2, PITCH = 132;
 };
 
-template <class T, int N> struct Vec;
-template <> struct Vec<_Float16, 8> { typedef h8 type; };
-template <> struct Vec<_Float16, 4> { typedef h4 type; };
-template <> struct Vec<_Float16, 2> { typedef h2 type; };
-template <> struct Vec<float, 4> { typedef f4 type; };
-template <> struct Vec<float, 2> { typedef f2 type; };
-
-__device__ __forceinline__ bool finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
-__device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000) != 0x7f800000; }
-
 template <class T, int DIMS, bool PAGED, bool BY_TOKEN>
 __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
     typedef Shape<T, DIMS> S;
@@ -99,19 +60,8 @@ __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
     const int part = x / across, who = x % across, b = col_tile / p.tiles, tile = col_tile % p.tiles;
     const int kv_head = BY_TOKEN ? who / group : who;
 
-    int len, count, row0, seq = b;
-    if (PAGED) {
-        if (b >= p.words.first[p.words.sequences + 1]) return;
-        seq = p.words.batch[b];
-        len = p.words.len[seq];
-        row0 = p.words.first[b];
-        count = min(p.words.first[b + 1], p.tokens) - row0;
-    } else {
-        len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-        count = p.tokens;   // (rows behind the length see nothing: zero)
-        row0 = 0;
-    }
-    const int pos0 = PAGED ? len - (p.words.first[b + 1] - row0) : 0;
+    const Batched in = batched<PAGED>(p, b);
+    const int len = in.len, count = in.count, row0 = in.row0, seq = in.seq, pos0 = in.pos0;
     const int token_tile = BY_TOKEN ? tile : tile / ((group + 15) / 16);
     const int tok = BY_TOKEN ? token_tile * 16 + c : token_tile;
     if ((BY_TOKEN ? token_tile * 16 : token_tile) >= count) return;
@@ -441,6 +391,7 @@ static void launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
 int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }
 
 int launch_attention(const AttnParams& p, hipStream_t s) {
+    if (p.tiled) return p.f16 ? launch_tiles_f16(p, s) : launch_tiles_f32(p, s);
     const int64_t across = p.by_token ? p.heads : p.kv_heads;
     const int64_t blocks = (across * p.parts + 7) / 8 * 8 * (int64_t)p.tiles * p.batch;
     if (blocks <= 0) return 0;

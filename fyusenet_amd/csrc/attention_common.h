@@ -1,0 +1,69 @@
+// What the attention kernels share: vector types, what a query sees, which rows a sequence of a batch has.
+#pragma once
+#include "sequence.h"
+
+#include <type_traits>
+
+namespace fynhip {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr float kNone = -__builtin_huge_valf();
+
+// The positions that one query sees: [lo, hi) and [0, first).
+struct Sight {
+    int lo, hi, first;
+    __device__ bool sees(int j) const { return (j >= lo && j < hi) || j < first; }
+};
+
+__device__ __forceinline__ Sight sight_of(int pos, int len, int causal, int window, int sinks) {
+    Sight s;
+    const int last = causal ? min(pos + 1, len) : len;
+    s.lo = 0; s.hi = last; s.first = 0;
+    if (window > 0) {
+        s.lo = max(0, pos - window + 1);
+        s.hi = (int)min((int64_t)last, (int64_t)pos + window);
+        s.first = min(sinks, last);
+    }
+    return s;
+}
+
+template <class T, int N> struct Vec;
+template <> struct Vec<_Float16, 8> { typedef h8 type; };
+template <> struct Vec<_Float16, 4> { typedef h4 type; };
+template <> struct Vec<_Float16, 2> { typedef h2 type; };
+template <> struct Vec<float, 4> { typedef f4 type; };
+template <> struct Vec<float, 2> { typedef f2 type; };
+
+__device__ __forceinline__ bool finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
+__device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000) != 0x7f800000; }
+
+// A sequence of the batch: its tokens, and its queries: `count` rows from row0 of q and the result, the first of them at
+// position pos0.
+struct Batched {
+    int seq, len, count, row0, pos0;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ Batched batched(const AttnParams& p, int b) {
+    Batched s{b, 0, 0, 0, 0};
+    if (PAGED) {
+        if (b >= p.words.first[p.words.sequences + 1]) return s;
+        s.seq = p.words.batch[b];
+        s.len = p.words.len[s.seq];
+        s.row0 = p.words.first[b];
+        const int end = p.words.first[b + 1];
+        s.count = min(end, p.tokens) - s.row0;
+        s.pos0 = s.len - (end - s.row0);
+    } else {
+        s.len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
+        s.count = p.tokens;   // (rows behind the length see nothing: zero)
+    }
+    return s;
+}
+
+}  // namespace fynhip

@@ -47,6 +47,19 @@ static void check_storage(int storage) {
     if (storage != FYN_STORAGE_F32 && storage != FYN_STORAGE_F16) fail(FYN_ERR_INVALID, "unknown storage type %d", storage);
 }
 
+// How many tokens of a head a workgroup of the kernel with tiles in shared memory gets; 0: the call is not for it.
+static int tiled(const AttnParams& p) {
+    if (!p.paged && std::max(p.k.tok, p.v.tok) * (p.f16 ? 2 : 4) > (1 << 24)) return 0;      // (32 bits of offset within a tile)
+    // Large workgroups read keys and values the fewest times, small ones are more: 128 queries where that gives workgroups
+    // for one and a half of the chip's CUs (16 heads of 4096 tokens: 108 us, against 150 with 64), 64 where it gives them for
+    // half of them (8 heads of 2048 tokens, two sequences: 52 us, against 61 with 128 and 121 without tiles).
+    const int64_t units = (int64_t)p.batch * p.heads;
+    auto fit = p.f16 ? tiles_fit_f16 : tiles_fit_f32;
+    if (units * ((p.tokens + 127) / 128) >= 384 && fit(p.dim, 128)) return 128;
+    if (units * ((p.tokens + 63) / 64) >= 128 && fit(p.dim, 64)) return 64;
+    return 0;
+}
+
 bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     check_storage(a.storage);
     check_heads(a.heads, a.kv_heads, a.head_dim);
@@ -73,9 +86,11 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     p.causal = a.causal != 0; p.window = a.window; p.sinks = a.sinks;
     p.scale_log2 = scale_log2(a.scale, a.head_dim);
     p.by_token = 1;
-    p.tiles = (a.tokens + 15) / 16;
     p.chunk = 0x7fffffff;
     p.parts = 1;
+    p.tiled = tiled(p);
+    const int columns = p.tiled ? p.tiled : 16;
+    p.tiles = (a.tokens + columns - 1) / columns;
     return true;
 }
 

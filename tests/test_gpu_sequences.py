@@ -97,6 +97,19 @@ PROMPTS = [
     (1, 190, 3, 3, 256, True, 70, 5, None),
     (1, 1100, 2, 2, 32, True, 300, 33, None),
     (5, 70, 16, 2, 128, True, 0, 0, [70, 69, 64, 1, 0]),
+    # enough heads and sequences for workgroups of 64 queries
+    (4, 260, 8, 2, 32, True, 0, 0, None),
+    (4, 261, 8, 4, 64, False, 50, 9, [261, 0, 130, 3]),
+    (3, 330, 12, 3, 96, True, 100, 70, [330, 65, 64]),
+    (2, 290, 16, 4, 128, False, 0, 0, [290, 258]),
+    (2, 270, 16, 8, 256, True, 33, 5, None),
+    (9, 70, 16, 2, 128, True, 0, 0, [70, 69, 64, 1, 0, 33, 70, 2, 65]),
+    # ... and of 128
+    (8, 300, 16, 4, 128, True, 0, 0, [300, 299, 257, 256, 128, 127, 1, 0]),
+    (8, 270, 16, 2, 32, False, 20, 40, None),
+    (8, 290, 16, 16, 64, True, 77, 3, [290, 129, 128, 65, 64, 63, 33, 290]),
+    (6, 400, 18, 6, 80, False, 0, 0, [400, 390, 130, 5, 1, 250]),
+    (6, 300, 24, 3, 200, True, 150, 140, None),
 ]
 
 
@@ -118,11 +131,11 @@ def test_prompt(case, typ):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("typ", ["f16", "f32"])
-@pytest.mark.parametrize("tokens,dim", [(150, 64), (600, 128)])
-def test_prompt_of_values_that_nobody_sees(typ, tokens, dim):
+@pytest.mark.parametrize("tokens,heads,dim", [(150, 2, 64), (600, 2, 128), (600, 16, 128), (600, 80, 64)])
+def test_prompt_of_values_that_nobody_sees(typ, tokens, heads, dim):
     """NaN and infinities behind a sequence's end, and in tokens that only later rows see."""
     n, bad = tokens - 20, tokens // 2
-    q, k, v = values(7, typ, (1, tokens, 2, dim), (1, tokens, 2, dim), (1, tokens, 2, dim))
+    q, k, v = values(7, typ, (1, tokens, heads, dim), (1, tokens, 2, dim), (1, tokens, 2, dim))
     lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
     clean = torch.empty_like(q)
     fa.attention(q, k, v, clean, lengths=lengths, window=37, sinks=3, stream=stream())
@@ -144,9 +157,9 @@ def test_prompt_of_values_that_nobody_sees(typ, tokens, dim):
         v3 = v.clone()
         v3[0, bad, 1] = math.inf
         fa.attention(q, k, v3, out, lengths=lengths, window=37, sinks=3, stream=stream())
-        assert torch.equal(out[0, :n, 0], clean[0, :n, 0])
+        assert torch.equal(out[0, :n, :heads // 2], clean[0, :n, :heads // 2])
         assert torch.equal(out[0, :n][untouched.cuda()], clean[0, :n][untouched.cuda()])
-        assert not torch.isfinite(out[0, bad:min(n, bad + 37), 1]).any()
+        assert not torch.isfinite(out[0, bad:min(n, bad + 37), heads // 2:]).any()
 
 
 @pytest.mark.gpu
