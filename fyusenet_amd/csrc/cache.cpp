@@ -202,40 +202,44 @@ void Cache::expect(int rows, hipStream_t s) {
     enter(s);
 }
 
-// Runs of changed words that lie one behind the other in a launch's argument; the order of the changes is kept.
-void Cache::flush(hipStream_t s) {
-    CacheUpdate u;
-    u.n = 0;
+// What the book has changed, on the device: words, lists that are copies of another's, pages that are copied; in as few launches
+// as their arguments hold.  The parts of a launch run in any order.  That is sound: a call changes no word twice, no page is
+// copied from and to, a list that is copied from or to has no words changed in the same call, and copies do not look at words.
+void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, int n, const int* lists) {
+    CacheChange c;
+    c.update = c.lists = c.moves = 0;
+    c.source = source;
+    c.entries = n > 0 ? (int)book_.list(lists[0]).size() : 0;
+    const CacheMemory m = memory();
     auto send = [&] {
-        if (!u.n) return;
-        launch_cache_update(words_, u, s);
-        u.n = 0;
+        if (c.any()) launch_cache_change(m, c, s);
+        c.update = c.lists = c.moves = 0;
     };
-    for (auto [at, end] : book_.changes()) {
+    // (words first: the others stand behind them in the argument)
+    for (auto [at, end] : book_.changes())
         while (at < end) {
-            if (u.n + 3 > kUpdateWords) send();
-            const int n = (int)std::min<size_t>(end - at, kUpdateWords - u.n - 2);
-            u.w[u.n] = (int)at;
-            u.w[u.n + 1] = n;
-            std::copy_n(book_.words.begin() + at, n, u.w + u.n + 2);
-            u.n += 2 + n;
-            at += n;
+            if (c.room() < 3) send();
+            const int k = (int)std::min<size_t>(end - at, c.room() - 2);
+            c.w[c.update] = (int)at;
+            c.w[c.update + 1] = k;
+            std::copy_n(book_.words.begin() + at, k, c.w + c.update + 2);
+            c.update += 2 + k;
+            at += k;
         }
+    book_.changes_taken();
+    for (int i = 0; i < n && c.entries > 0; i++) {
+        if (c.room() < 1) send();
+        c.w[c.update + c.lists++] = lists[i];
+    }
+    // (a launch has at most 2^31 workgroups)
+    const int64_t most = std::max<int64_t>(1, (int64_t)0x7fff0000 / (page_bytes_ / 16384 + 1));
+    for (const auto& x : moves) {
+        if (c.room() < 2 || c.moves >= most) send();
+        c.w[c.update + c.lists + 2 * c.moves] = x.first;
+        c.w[c.update + c.lists + 2 * c.moves + 1] = x.second;
+        c.moves++;
     }
     send();
-    book_.changes_taken();
-    FYN_HIP(hipGetLastError());
-}
-
-void Cache::move(const PageBook::Moves& m, hipStream_t s) {
-    PageCopies c;
-    for (size_t i = 0; i < m.size();) {
-        for (c.n = 0; c.n < kPageCopies && i < m.size(); c.n++, i++) {
-            c.from[c.n] = m[i].first;
-            c.to[c.n] = m[i].second;
-        }
-        launch_page_copies(pool_, page_bytes_, c, s);
-    }
     FYN_HIP(hipGetLastError());
 }
 
@@ -268,8 +272,7 @@ void Cache::extend(int n, const int* seqs, const int* counts, hipStream_t s) {
     if (n > 0 && !counts) fail(FYN_ERR_INVALID, "cache: no numbers of tokens given");
     OnDevice on(device);
     settle(s);
-    move(booked([&] { return book_.extend(n, seqs, counts); }), s);
-    flush(s);
+    carry_out(booked([&] { return book_.extend(n, seqs, counts); }), s);
 }
 
 void Cache::fork(int source, int n, const int* targets, int tokens, hipStream_t s) {
@@ -277,15 +280,7 @@ void Cache::fork(int source, int n, const int* targets, int tokens, hipStream_t 
     OnDevice on(device);
     settle(s);
     booked([&] { book_.fork(source, n, targets, tokens); return 0; });
-    if (n > 0) {
-        RowCopies r;
-        r.words = (int)book_.list(targets[0]).size();
-        for (int i = 0; i < n && r.words > 0;) {
-            for (r.n = 0; r.n < kRowCopies && i < n; r.n++, i++) r.to[r.n] = targets[i];
-            launch_row_copies(words_ + book_.table_at(), book_.pitch(), source, r, s);
-        }
-    }
-    flush(s);
+    carry_out({}, s, source, n, targets);
 }
 
 void Cache::copy(int n, const int* sources, const int* targets, hipStream_t s) {
@@ -293,8 +288,7 @@ void Cache::copy(int n, const int* sources, const int* targets, hipStream_t s) {
     if (n > 0 && !sources) fail(FYN_ERR_INVALID, "cache: no sequences given");
     OnDevice on(device);
     settle(s);
-    move(booked([&] { return book_.copy(n, sources, targets); }), s);
-    flush(s);
+    carry_out(booked([&] { return book_.copy(n, sources, targets); }), s);
 }
 
 void Cache::truncate(int n, const int* seqs, const int* tokens, hipStream_t s) {
@@ -302,15 +296,14 @@ void Cache::truncate(int n, const int* seqs, const int* tokens, hipStream_t s) {
     OnDevice on(device);
     settle(s);
     booked([&] { book_.truncate(n, seqs, tokens); return 0; });
-    flush(s);
+    carry_out({}, s);
 }
 
 void Cache::compact(int* used, hipStream_t s) {
     std::lock_guard<std::mutex> lock(mu_);
     OnDevice on(device);
     settle(s);
-    move(book_.compact(), s);
-    flush(s);
+    carry_out(book_.compact(), s);
     if (used) *used = book_.pages_used();
 }
 

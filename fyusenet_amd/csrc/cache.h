@@ -46,8 +46,8 @@ class Cache : public std::enable_shared_from_this<Cache> {
     bool enter(hipStream_t s);     // -> the stream is being captured
     void settle(hipStream_t s);    // no capture: what changes on the host cannot be replayed
     void join_streams(hipStream_t s);
-    void flush(hipStream_t s);
-    void move(const PageBook::Moves& m, hipStream_t s);
+    CacheMemory memory() const { return CacheMemory{words_, words_ + book_.table_at(), book_.pitch(), pool_, page_bytes_}; }
+    void carry_out(const PageBook::Moves& moves, hipStream_t s, int source = 0, int n = 0, const int* lists = nullptr);
     PageLayout layout(int layer) const;
     CacheWords words() const;
 };

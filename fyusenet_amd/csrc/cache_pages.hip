@@ -6,41 +6,62 @@ namespace fynhip {
 
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
-// Changed words travel as the launch's argument: no host memory has to outlive the call, and nothing is copied between
-// host and device on the way.
-__global__ __launch_bounds__(256) void update_words(int* __restrict__ words, const CacheUpdate u) {
-    for (int i = 0; i < u.n;) {
-        const int at = u.w[i], n = u.w[i + 1];
-        for (int k = threadIdx.x; k < n; k += 256) words[at + k] = u.w[i + 2 + k];
-        i += 2 + n;
+template <int WORDS>
+struct ChangeArgument {
+    int update, lists, moves, source, entries;
+    int w[WORDS];
+};
+
+// One launch for all that a call changes.  Workgroup 0 writes the words, the next ones the lists, the others copy pages, each a
+// part of one: 16 KB, four vectors of 16 bytes a thread.
+constexpr int kPart = 16 << 10;
+template <int WORDS>
+__global__ __launch_bounds__(256) void change_cache(const CacheMemory m, const ChangeArgument<WORDS> c, const int parts) {
+    int b = blockIdx.x;
+    if (b == 0) {
+        for (int i = 0; i < c.update;) {
+            const int at = c.w[i], n = c.w[i + 1];
+            for (int k = threadIdx.x; k < n; k += 256) m.words[at + k] = c.w[i + 2 + k];
+            i += 2 + n;
+        }
+        return;
     }
+    b -= 1;
+    if (b < c.lists) {
+        const int* src = m.table + (int64_t)c.source * m.pitch;
+        int* dst = m.table + (int64_t)c.w[c.update + b] * m.pitch;
+        for (int i = threadIdx.x; i < c.entries; i += 256) dst[i] = src[i];
+        return;
+    }
+    b -= c.lists;
+    const int pair = b / parts;
+    const int64_t at = (int64_t)(b % parts) * kPart;
+    const char* src = m.pool + c.w[c.update + c.lists + 2 * pair] * m.page_bytes + at;
+    char* dst = m.pool + c.w[c.update + c.lists + 2 * pair + 1] * m.page_bytes + at;
+    const int64_t left = m.page_bytes - at;
+    u4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if ((i * 256 + threadIdx.x) * 16 < left) v[i] = *reinterpret_cast<const u4*>(src + (i * 256 + threadIdx.x) * 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if ((i * 256 + threadIdx.x) * 16 < left) *reinterpret_cast<u4*>(dst + (i * 256 + threadIdx.x) * 16) = v[i];
 }
 
-void launch_cache_update(int* words, const CacheUpdate& u, hipStream_t s) {
-    hipLaunchKernelGGL(update_words, dim3(1), dim3(256), 0, s, words, u);
+template <int WORDS>
+static void launch_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
+    ChangeArgument<WORDS> a;
+    a.update = c.update; a.lists = c.lists; a.moves = c.moves; a.source = c.source; a.entries = c.entries;
+    const int n = c.update + c.lists + 2 * c.moves;
+    for (int i = 0; i < n; i++) a.w[i] = c.w[i];
+    const int64_t parts = (m.page_bytes + kPart - 1) / kPart;
+    hipLaunchKernelGGL(change_cache<WORDS>, dim3((unsigned)(1 + c.lists + c.moves * parts)), dim3(256), 0, s, m, a, (int)parts);
 }
 
-__global__ __launch_bounds__(256) void copy_rows(int* __restrict__ table, int pitch, int from, const RowCopies r) {
-    const int* src = table + (int64_t)from * pitch;
-    int* dst = table + (int64_t)r.to[blockIdx.y] * pitch;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < r.words; i += gridDim.x * 256) dst[i] = src[i];
-}
-
-void launch_row_copies(int* table, int pitch, int from, const RowCopies& r, hipStream_t s) {
-    const unsigned x = (unsigned)min((r.words + 255) / 256, 64);
-    hipLaunchKernelGGL(copy_rows, dim3(x, (unsigned)r.n), dim3(256), 0, s, table, pitch, from, r);
-}
-
-__global__ __launch_bounds__(256) void copy_pages(char* __restrict__ pool, int64_t page_bytes, const PageCopies c) {
-    const u4* src = reinterpret_cast<const u4*>(pool + c.from[blockIdx.y] * page_bytes);
-    u4* dst = reinterpret_cast<u4*>(pool + c.to[blockIdx.y] * page_bytes);
-    const int64_t n = page_bytes / 16;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) dst[i] = src[i];
-}
-
-void launch_page_copies(char* pool, int64_t page_bytes, const PageCopies& c, hipStream_t s) {
-    const int64_t x = (page_bytes / 16 + 1023) / 1024;   // four vectors a thread
-    hipLaunchKernelGGL(copy_pages, dim3((unsigned)(x < 1 ? 1 : x > 256 ? 256 : x), (unsigned)c.n), dim3(256), 0, s, pool, page_bytes, c);
+void launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
+    const int n = c.update + c.lists + 2 * c.moves;
+    if (n <= 48) launch_change<48>(m, c, s);
+    else launch_change<kChangeWords>(m, c, s);
 }
 
 // where the head's keys of a token of a sequence are

@@ -63,24 +63,28 @@ bool tiles_fit_f16(int dim, int queries);                   // whether there is 
 bool tiles_fit_f32(int dim, int queries);
 int attention_step(int f16, int dim);   // keys of one step of the kernel (AttnParams::chunk counts them)
 
-constexpr int kUpdateWords = 896;
-struct CacheUpdate {        // (a kernel argument: at most 4 KB of them)
-    int n;
-    int w[kUpdateWords];    // {first word, number of words, words ...} ...
+// What the host changes of a cache in one launch.  It travels as the kernel's argument (at most 4 KB, and 256 bytes where it is
+// little: the argument's size is part of a launch's time): no memory of the host's has to outlive the call.
+// Words: {first word, number of words, words ...} ...; lists of pages that become copies of another's first entries; pages
+// that are copied.
+constexpr int kChangeWords = 960;
+struct CacheChange {
+    int update;             // words of the first kind in w, from 0
+    int lists;              // sequences in w behind them, whose lists become copies of the first `entries` of `source`'s
+    int moves;              // pairs {from, to} in w behind those
+    int source, entries;
+    int w[kChangeWords];
+    int room() const { return kChangeWords - update - lists - 2 * moves; }
+    bool any() const { return update || lists || moves; }
 };
-void launch_cache_update(int* words, const CacheUpdate& u, hipStream_t s);
-constexpr int kRowCopies = 896;
-struct RowCopies {
-    int n, words;
-    int to[kRowCopies];
+struct CacheMemory {
+    int* words;
+    int* table;
+    int pitch;
+    char* pool;
+    int64_t page_bytes;
 };
-void launch_row_copies(int* table, int pitch, int from, const RowCopies& r, hipStream_t s);
-constexpr int kPageCopies = 448;
-struct PageCopies {
-    int n;
-    int from[kPageCopies], to[kPageCopies];
-};
-void launch_page_copies(char* pool, int64_t page_bytes, const PageCopies& c, hipStream_t s);
+void launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s);
 
 struct CacheRows {          // tokens between a cache and tensors
     SeqRows k, v;

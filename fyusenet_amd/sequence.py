@@ -5,6 +5,7 @@ with __cuda_array_interface__, a capi.TensorView as custom layers get them, or a
 an integer (torch.cuda.current_stream().cuda_stream), 0 the default stream.  Calls return before the work is done.
 """
 import ctypes
+import struct
 
 import numpy as np
 
@@ -53,51 +54,99 @@ class DeviceArray:
 
 
 _TYPES = {capi.STORAGE_F16: "float16", capi.STORAGE_F32: "float32"}
+_STORAGES = {"float16": capi.STORAGE_F16, "float32": capi.STORAGE_F32}
+
+# The structs of the calls that a step makes, packed at once (field by field takes longer than the launch).
+_ROWS = "Q3q"
+_ATTENTION = struct.Struct("=I9if4xQ" + 4 * _ROWS)
+_ATTEND = struct.Struct("=I3if4x" + 2 * _ROWS)
+_ONE = struct.Struct("=" + _ROWS)
+assert _ATTENTION.size == ctypes.sizeof(capi.AttentionDesc) and _ATTEND.size == ctypes.sizeof(capi.AttendDesc) and _ONE.size == ctypes.sizeof(capi.Rows)
+
+_V = ctypes.c_void_p
+_calls = {}
 
 
-def _rows(a, name, storage, shape, r):
-    """Fills the Rows `r` with tensor `a` of shape [.., token, head, dim]."""
-    if a.dtype != _TYPES[storage]:
-        raise capi.FynException(capi.ERR_INVALID, "%s: %s values, %s are expected" % (name, a.dtype, _TYPES[storage]))
-    if tuple(a.shape) != shape:
-        raise capi.FynException(capi.ERR_INVALID, "%s: shape %s, %s is expected" % (name, tuple(a.shape), shape))
-    st = a.strides
+def _call(name, *args):
+    """An entry point that takes packed structs (bytes) where its prototype has pointers to them."""
+    fn = _calls.get(name)
+    if fn is None:
+        capi.lib()
+        fn = _calls[name] = ctypes.CFUNCTYPE(ctypes.c_int, *args)((name, capi.lib()))
+    return fn
+
+
+_dtypes = {}   # element types of tensors that have been seen -> their names
+
+
+def _take(x, name, heads=0):
+    """Address, element type, shape and strides of a tensor."""
+    try:
+        known = _dtypes.get(x.dtype)
+        if known is None:
+            known = _dtypes[x.dtype] = str(x.dtype).rpartition(".")[2]
+        if x.is_cuda:
+            return x.data_ptr(), known, x.shape, x.stride()
+    except (AttributeError, TypeError):
+        pass
+    a = DeviceArray.of(x, name, heads)
+    return a.ptr, a.dtype, a.shape, a.strides
+
+
+def _rows(a, name, typ, shape):
+    """Address and pitches (sequence, token, head) of a tensor [.., token, head, dim] that has to have this type and shape."""
+    ptr, dtype, have, st = a
+    if dtype != typ:
+        raise capi.FynException(capi.ERR_INVALID, "%s: %s values, %s are expected" % (name, dtype, typ))
+    if have != shape and tuple(have) != tuple(shape):
+        raise capi.FynException(capi.ERR_INVALID, "%s: shape %s, %s is expected" % (name, tuple(have), tuple(shape)))
     if st[-1] != 1 and shape[-1] > 1:
         raise capi.FynException(capi.ERR_INVALID, "%s: the values of a head have to lie side by side" % name)
     # (a distance that nothing is multiplied with may be anything)
-    r.data, r.head_pitch, r.token_pitch = a.ptr, st[-2] if shape[-2] > 1 else 0, st[-3] if shape[-3] > 1 else 0
-    r.sequence_pitch = st[0] if len(shape) == 4 and shape[0] > 1 else 0
+    return (ptr, st[0] if len(shape) == 4 and shape[0] > 1 else 0, st[-3] if shape[-3] > 1 else 0, st[-2] if shape[-2] > 1 else 0)
 
 
 def attention(queries, keys, values, result, lengths=None, causal=True, window=0, sinks=0, scale=0.0, heads=0, kv_heads=0, stream=0):
     """fyn_attention: queries and result [batch, tokens, heads, dim], keys and values [batch, tokens, kv_heads, dim].
     lengths: int32 [batch] or None.  heads and kv_heads are asked for only where tensors are given as TensorViews, whose
     rows are the sequences."""
-    q, k = DeviceArray.of(queries, "queries", heads), DeviceArray.of(keys, "keys", kv_heads or heads)
-    v, out = DeviceArray.of(values, "values", kv_heads or heads), DeviceArray.of(result, "result", heads)
-    if len(q.shape) != 4 or len(k.shape) != 4:
+    q, k = _take(queries, "queries", heads), _take(keys, "keys", kv_heads or heads)
+    shape, kv_shape = q[2], k[2]
+    if len(shape) != 4 or len(kv_shape) != 4:
         raise capi.FynException(capi.ERR_INVALID, "attention: tensors [batch, tokens, heads, dim] are expected")
-    d = capi.AttentionDesc()
-    d.struct_size = ctypes.sizeof(d)
-    d.storage = capi.STORAGE_F16 if q.dtype == "float16" else capi.STORAGE_F32
-    d.batch, d.tokens, d.heads, d.head_dim = q.shape
-    d.kv_heads = k.shape[2]
-    shape, kv_shape = tuple(q.shape), (q.shape[0], q.shape[1], k.shape[2], q.shape[3])
-    _rows(q, "queries", d.storage, shape, d.queries)
-    _rows(k, "keys", d.storage, kv_shape, d.keys)
-    _rows(v, "values", d.storage, kv_shape, d.values)
-    _rows(out, "result", d.storage, shape, d.result)
+    batch, tokens, nheads, dim = shape
+    typ = q[1]
+    kv_shape = (batch, tokens, kv_shape[2], dim)
+    storage = _STORAGES.get(typ)
+    if storage is None:
+        raise capi.FynException(capi.ERR_INVALID, "queries: %s values are not supported" % typ)
+    at = 0
     if lengths is not None:
-        n = DeviceArray.of(lengths, "lengths")
-        if n.dtype != "int32" or tuple(n.shape) != shape[:1] or (shape[0] > 1 and n.strides[0] != 1):
-            raise capi.FynException(capi.ERR_INVALID, "lengths: %d int32 values side by side are expected" % shape[0])
-        d.lengths = n.ptr
-    d.causal, d.window, d.sinks, d.scale = 1 if causal else 0, window, sinks, scale
-    capi.check(capi.lib().fyn_attention(ctypes.byref(d), stream))
+        n = _take(lengths, "lengths")
+        if n[1] != "int32" or tuple(n[2]) != (batch,) or (batch > 1 and n[3][0] != 1):
+            raise capi.FynException(capi.ERR_INVALID, "lengths: %d int32 values side by side are expected" % batch)
+        at = n[0]
+    try:
+        d = _ATTENTION.pack(_ATTENTION.size, storage, batch, tokens, nheads, kv_shape[2], dim, 1 if causal else 0, window, sinks, scale, at,
+                            *_rows(q, "queries", typ, shape), *_rows(k, "keys", typ, kv_shape),
+                            *_rows(_take(values, "values", kv_heads or heads), "values", typ, kv_shape),
+                            *_rows(_take(result, "result", heads), "result", typ, shape))
+    except (struct.error, OverflowError) as e:
+        raise capi.FynException(capi.ERR_INVALID, "attention: %s" % e)
+    status = _call("fyn_attention", _V, _V)(d, stream)
+    if status:
+        capi.check(status)
+
+
+_arrays = {}
 
 
 def _ints(v):
-    return (ctypes.c_int32 * len(v))(*v)
+    n = len(v)
+    t = _arrays.get(n)
+    if t is None:
+        t = _arrays[n] = ctypes.c_int32 * n
+    return t(*v)
 
 
 class SequenceCache:
@@ -114,6 +163,7 @@ class SequenceCache:
         capi.check(capi.lib().fyn_cache_create(device, ctypes.byref(d), ctypes.byref(self._h)))
         self.storage, self.layers, self.heads, self.kv_heads, self.head_dim = storage, layers, heads, kv_heads, head_dim
         self.page_tokens, self.sequences = page_tokens, sequences
+        self._type = _TYPES[storage]
 
     def _same(self, a, b, what):
         if len(a) != len(b):
@@ -124,30 +174,31 @@ class SequenceCache:
         capi.check(capi.lib().fyn_cache_extend(self._h, len(sequences), _ints(sequences), _ints(tokens), stream))
 
     def _kv(self, keys, values):
-        k, v = DeviceArray.of(keys, "keys"), DeviceArray.of(values, "values")
-        shape = (k.shape[0] if len(k.shape) == 3 else 0, self.kv_heads, self.head_dim)
-        rk, rv = capi.Rows(), capi.Rows()
-        _rows(k, "keys", self.storage, shape, rk)
-        _rows(v, "values", self.storage, shape, rv)
-        return rk, rv, shape[0]
+        k = _take(keys, "keys")
+        shape = (k[2][0] if len(k[2]) == 3 else 0, self.kv_heads, self.head_dim)
+        return _ONE.pack(*_rows(k, "keys", self._type, shape)), _ONE.pack(*_rows(_take(values, "values"), "values", self._type, shape)), shape[0]
 
     def write(self, layer, keys, values, stream=0):
-        rk, rv, rows = self._kv(keys, values)
-        capi.check(capi.lib().fyn_cache_write(self._h, layer, ctypes.byref(rk), ctypes.byref(rv), rows, stream))
+        k, v, rows = self._kv(keys, values)
+        capi.check(_call("fyn_cache_write", _V, ctypes.c_int, _V, _V, ctypes.c_int, _V)(self._h, layer, k, v, rows, stream))
 
     def attend(self, layer, queries, result, window=0, sinks=0, scale=0.0, stream=0):
-        q, out = DeviceArray.of(queries, "queries"), DeviceArray.of(result, "result")
-        shape = (q.shape[0] if len(q.shape) == 3 else 0, self.heads, self.head_dim)
-        d = capi.AttendDesc()
-        d.struct_size, d.rows, d.window, d.sinks, d.scale = ctypes.sizeof(d), shape[0], window, sinks, scale
-        _rows(q, "queries", self.storage, shape, d.queries)
-        _rows(out, "result", self.storage, shape, d.result)
-        capi.check(capi.lib().fyn_cache_attend(self._h, layer, ctypes.byref(d), stream))
+        q = _take(queries, "queries")
+        shape = (q[2][0] if len(q[2]) == 3 else 0, self.heads, self.head_dim)
+        try:
+            d = _ATTEND.pack(_ATTEND.size, shape[0], window, sinks, scale, *_rows(q, "queries", self._type, shape),
+                             *_rows(_take(result, "result"), "result", self._type, shape))
+        except (struct.error, OverflowError) as e:
+            raise capi.FynException(capi.ERR_INVALID, "attend: %s" % e)
+        status = _call("fyn_cache_attend", _V, ctypes.c_int, _V, _V)(self._h, layer, d, stream)
+        if status:
+            capi.check(status)
 
     def read(self, sequences, layer, keys, values, stream=0):
         """Keys and values of whole sequences into [tokens of all of them, kv_heads, dim]."""
-        rk, rv, rows = self._kv(keys, values)
-        capi.check(capi.lib().fyn_cache_read(self._h, len(sequences), _ints(sequences), layer, ctypes.byref(rk), ctypes.byref(rv), rows, stream))
+        k, v, rows = self._kv(keys, values)
+        capi.check(_call("fyn_cache_read", _V, ctypes.c_int, _V, ctypes.c_int, _V, _V, ctypes.c_int, _V)(
+            self._h, len(sequences), _ints(sequences), layer, k, v, rows, stream))
 
     def fork(self, source, targets, tokens=-1, stream=0):
         capi.check(capi.lib().fyn_cache_fork(self._h, source, len(targets), _ints(targets), tokens, stream))
