@@ -31,6 +31,8 @@ struct Shape {
     static constexpr int KLOADS = DIMS / (4 * VEC);               // ... for one key: 4 lanes side by side
     static constexpr int TILES = (!F16 && DIMS > 128) ? 1 : 2;    // sixteens of keys in a step
     static constexpr int STEP = 16 * TILES;
+    static constexpr int WAVES = F16 && DIMS <= 128 ? 3 : DIMS <= 64 ? 3 : DIMS <= 128 ? 2 : 1;   // workgroups that share a CU
+    static constexpr int LEAST = DIMS == 32 ? 0 : DIMS == 256 ? 128 : DIMS - 32;   // fewer dims than any head of the class has
     static constexpr int E = DIMS / 16 < VEC ? DIMS / 16 : VEC;   // dims that a lane loads of V at once
     static constexpr int BLOCKS = (DIMS + 16 * E - 1) / (16 * E);
     static constexpr int PITCH = BLOCKS * 16 * E + 4;             // of the joined sums in LDS (floats)
@@ -40,16 +42,21 @@ struct Shape {
 template <class T>
 struct Shape<T, 96> {
     static constexpr bool F16 = std::is_same<T, _Float16>::value;
-    static constexpr int VEC = 16 / sizeof(T), KLOADS = 96 / (4 * VEC), TILES = 2, STEP = 32, E = F16 ? 8 : 4, BLOCKS = F16 ? 1 : 2, PITCH = 132;
+    static constexpr int VEC = 16 / sizeof(T), KLOADS = 96 / (4 * VEC), TILES = 2, STEP = 32, LEAST = 64, WAVES = F16 ? 3 : 2, E = F16 ? 8 : 4, BLOCKS = F16 ? 1 : 2, PITCH = 132;
 };
 
-template <class T, int DIMS, bool PAGED, bool BY_TOKEN>
-__global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
+template <bool ONCE, class V>
+__device__ __forceinline__ V load(const void* p) {
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const V*>(p)) : *reinterpret_cast<const V*>(p);
+}
+
+template <class T, int DIMS, bool PAGED, bool BY_TOKEN, bool ONCE>
+__global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(const AttnParams p) {
     typedef Shape<T, DIMS> S;
     typedef typename Vec<T, S::VEC>::type KVec;
     typedef typename Vec<T, S::E>::type VVec;
     constexpr bool F16 = S::F16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
 
     // Which part of which columns.  Workgroups that read the same keys for different sequences (branches of one sequence
     // share pages) or columns lie eight apart, which is on one XCD and its L2, one behind the other.
@@ -117,46 +124,71 @@ __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
     }
     const int* table = PAGED ? p.words.table + (int64_t)seq * p.words.table_pitch : nullptr;
 
-    for (int st = begin + wave; st < end; st += 4) {
-        const int at = (st < a_steps ? st : b_first + st - a_steps) * S::STEP;
-        int page[4] = {0, 0, 0, 0};
+    // Where a step's keys and values are for this lane: those of key 16 t + c, piece g, and of the keys 16 t + 4 g .. + 3,
+    // dims from c E on.  Pages have eight tokens or more: half a sixteen lies in one.  A list is not read behind its last page;
+    // what is read behind the last visible key is within a page (or, nothing paged, the last visible key again).
+    struct Where {
+        const char *k[S::TILES], *v[S::TILES];
+        int rows[S::TILES];   // nothing paged: how many keys from the lane's first value's there are, less one
+    };
+    const int row_bytes = p.dim * (int)sizeof(T);
+    auto at_of = [&](int st) { return (st < a_steps ? st : b_first + st - a_steps) * S::STEP; };
+    auto where = [&](int at) {
+        Where w;
         if (PAGED) {
-            const int top = (most - 1) >> p.pages.shift;
+            const int top = (most - 1) >> p.pages.shift, mask = (1 << p.pages.shift) - 1;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i == 0 || (S::STEP >> p.pages.shift) > i) page[i] = table[min((at >> p.pages.shift) + i, top)];
-        }
-        auto row = [&](const char* base, int64_t tok_pitch, int off) -> const T* {   // of the key at + off; none behind the last visible one is read
-            const int j = min(at + off, most - 1);
-            if (PAGED) {
-                const int i = (j >> p.pages.shift) - (at >> p.pages.shift);
-                const int pg = i == 0 ? page[0] : i == 1 ? page[1] : i == 2 ? page[2] : page[3];
-                return reinterpret_cast<const T*>(base + pg * p.pages.page_bytes) + (j & ((1 << p.pages.shift) - 1)) * p.dim;
+            for (int t = 0; t < S::TILES; t++) {
+                const int64_t a = table[min((at + 16 * t) >> p.pages.shift, top)] * p.pages.page_bytes, b = table[min((at + 16 * t + 8) >> p.pages.shift, top)] * p.pages.page_bytes;
+                w.k[t] = kbase + (c < 8 ? a : b) + ((at + 16 * t + c) & mask) * row_bytes;
+                w.v[t] = vbase + (g < 2 ? a : b) + ((at + 16 * t + 4 * g) & mask) * row_bytes;
+                w.rows[t] = 3;
             }
-            return reinterpret_cast<const T*>(base) + j * tok_pitch;
-        };
-        KVec k[S::TILES][S::KLOADS];
-        VVec v[S::TILES][4][S::BLOCKS];
+        } else {
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            const T* src = row(kbase, p.k.tok, 16 * t + c);
-#pragma unroll
-            for (int s = 0; s < S::KLOADS; s++) {
-                const int d = (s * 4 + g) * S::VEC;
-                k[t][s] = d < p.dim ? *reinterpret_cast<const KVec*>(src + d) : KVec{};
+            for (int t = 0; t < S::TILES; t++) {
+                w.k[t] = kbase + min(at + 16 * t + c, most - 1) * p.k.tok * (int64_t)sizeof(T);
+                const int j = min(at + 16 * t + 4 * g, most - 1);
+                w.v[t] = vbase + j * p.v.tok * (int64_t)sizeof(T);
+                w.rows[t] = most - 1 - j;
             }
         }
+        return w;
+    };
+    const int64_t v_pitch = PAGED ? row_bytes : p.v.tok * (int64_t)sizeof(T);
+    KVec k[S::TILES][S::KLOADS];
+    VVec v[S::TILES][4][S::BLOCKS];
+    // (pieces behind a head's last value are taken from within it: they meet queries that are zero, or end in dims that nobody stores)
+    auto load_keys = [&](const Where& w) {
 #pragma unroll
         for (int t = 0; t < S::TILES; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const T* src = row(vbase, p.v.tok, 16 * t + 4 * g + r);
+            for (int s = 0; s < S::KLOADS; s++) {
+                const int at = (s * 4 + g) * 16;
+                k[t][s] = load<ONCE, KVec>(w.k[t] + ((s + 1) * 4 * S::VEC <= S::LEAST ? at : min(at, row_bytes - 16)));
+            }
+    };
+    auto load_values = [&](const Where& w) {
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int i = 0; i < S::BLOCKS; i++) {
-                    const int d = (i * 16 + c) * S::E;
-                    v[t][r][i] = d < p.dim ? *reinterpret_cast<const VVec*>(src + d) : VVec{};
+                    const int at = (i * 16 + c) * S::E * (int)sizeof(T);
+                    v[t][r][i] = load<ONCE, VVec>(w.v[t] + min(r, w.rows[t]) * v_pitch + min(at, row_bytes - S::E * (int)sizeof(T)));
                 }
-            }
+    };
+    // The next step's keys are asked for when this one's have gone through the first product, its values when these have gone
+    // through the second.
+    if (begin + wave < end) {
+        const Where w = where(at_of(begin + wave));
+        load_keys(w);
+        load_values(w);
+    }
+    for (int st = begin + wave; st < end; st += 4) {
+        const int at = at_of(st);
+        const Where next = where(at_of(min(st + 4, end - 1)));
         // scores
         f4 sc[S::TILES];
 #pragma unroll
@@ -173,6 +205,7 @@ __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
             }
             sc[t] *= p.scale_log2;
         }
+        if (st + 4 < end) load_keys(next);
         // Whether every column sees every key of the step; if not, what a column does not see weighs nothing, whatever
         // the memory holds there.
         const bool whole = (at >= all.lo && at + S::STEP <= all.hi) || at + S::STEP <= all.first;
@@ -261,7 +294,9 @@ __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
                     for (int rr = 0; rr < 4; rr++)
                         if (tt == t && rr == r) weight = w[tt][rr];
                 weight = __shfl(weight, owner * 16 + c);
-                const T* src = row(vbase, p.v.tok, off);
+                const int j = min(at + off, most - 1);
+                const T* src = reinterpret_cast<const T*>(PAGED ? vbase + table[j >> p.pages.shift] * p.pages.page_bytes + (j & ((1 << p.pages.shift) - 1)) * row_bytes
+                                                                : vbase + j * p.v.tok * (int64_t)sizeof(T));
 #pragma unroll
                 for (int i = 0; i < S::BLOCKS; i++)
 #pragma unroll
@@ -276,6 +311,7 @@ __global__ __launch_bounds__(256) void attend_steps(const AttnParams p) {
                         }
             }
         }
+        if (st + 4 < end) load_values(next);
     }
 
     // the four waves' sums: each has a maximum of its own
@@ -380,10 +416,11 @@ __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
 template <class T, int DIMS>
 static void launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
     if (p.paged) {
-        if (p.by_token) hipLaunchKernelGGL((attend_steps<T, DIMS, true, true>), dim3(blocks), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((attend_steps<T, DIMS, true, false>), dim3(blocks), dim3(256), 0, s, p);
+        if (p.by_token) hipLaunchKernelGGL((attend_steps<T, DIMS, true, true, false>), dim3(blocks), dim3(256), 0, s, p);
+        else if (p.once) hipLaunchKernelGGL((attend_steps<T, DIMS, true, false, true>), dim3(blocks), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((attend_steps<T, DIMS, true, false, false>), dim3(blocks), dim3(256), 0, s, p);
     } else {
-        hipLaunchKernelGGL((attend_steps<T, DIMS, false, true>), dim3(blocks), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((attend_steps<T, DIMS, false, true, false>), dim3(blocks), dim3(256), 0, s, p);
     }
     if (p.parts > 1) hipLaunchKernelGGL((join_parts<T, DIMS>), dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, s, p);
 }

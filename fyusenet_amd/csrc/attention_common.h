@@ -52,11 +52,13 @@ template <bool PAGED>
 __device__ __forceinline__ Batched batched(const AttnParams& p, int b) {
     Batched s{b, 0, 0, 0, 0};
     if (PAGED) {
-        if (b >= p.words.first[p.words.sequences + 1]) return s;
-        s.seq = p.words.batch[b];
-        s.len = p.words.len[s.seq];
-        s.row0 = p.words.first[b];
-        const int end = p.words.first[b + 1];
+        // (everything that does not wait for another is asked for at once; b is within the tables)
+        const int n = p.words.first[p.words.sequences + 1], seq = p.words.batch[b], row0 = p.words.first[b], end = p.words.first[b + 1];
+        const int len = p.words.len[seq];
+        if (b >= n) return s;
+        s.seq = seq;
+        s.len = len;
+        s.row0 = row0;
         s.count = min(end, p.tokens) - s.row0;
         s.pos0 = s.len - (end - s.row0);
     } else {

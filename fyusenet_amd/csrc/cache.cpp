@@ -206,37 +206,48 @@ void Cache::expect(int rows, hipStream_t s) {
 // as their arguments hold.  The parts of a launch run in any order.  That is sound: a call changes no word twice, no page is
 // copied from and to, a list that is copied from or to has no words changed in the same call, and copies do not look at words.
 void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, int n, const int* lists) {
+    const CacheMemory m = memory();
     CacheChange c;
-    c.update = c.lists = c.moves = 0;
+    auto clear = [&] { c.runs = c.singles = c.lists = c.moves = 0; };
+    auto send = [&] {
+        if (c.used()) launch_cache_change(m, c, s);
+        clear();
+    };
+    clear();
     c.source = source;
     c.entries = n > 0 ? (int)book_.list(lists[0]).size() : 0;
-    const CacheMemory m = memory();
-    auto send = [&] {
-        if (c.any()) launch_cache_change(m, c, s);
-        c.update = c.lists = c.moves = 0;
-    };
-    // (words first: the others stand behind them in the argument)
+    constexpr size_t kFew = 4;   // words of a run that go one by one: all at once then, where runs wait for each other's lengths
     for (auto [at, end] : book_.changes())
-        while (at < end) {
-            if (c.room() < 3) send();
-            const int k = (int)std::min<size_t>(end - at, c.room() - 2);
-            c.w[c.update] = (int)at;
-            c.w[c.update + 1] = k;
-            std::copy_n(book_.words.begin() + at, k, c.w + c.update + 2);
-            c.update += 2 + k;
+        while (end - at > kFew) {
+            if (c.used() + 3 > kChangeWords) send();
+            const int k = (int)std::min<size_t>(end - at, kChangeWords - c.used() - 2);
+            c.w[c.runs] = (int)at;
+            c.w[c.runs + 1] = k;
+            std::copy_n(book_.words.begin() + at, k, c.w + c.runs + 2);
+            c.runs += 2 + k;
             at += k;
         }
+    for (auto [at, end] : book_.changes()) {
+        if (end - at > kFew) continue;
+        for (; at < end; at++) {
+            if (c.used() + 2 > kChangeWords) send();
+            c.w[c.used()] = (int)at;
+            c.w[c.used() + 1] = book_.words[at];
+            c.singles++;
+        }
+    }
     book_.changes_taken();
     for (int i = 0; i < n && c.entries > 0; i++) {
-        if (c.room() < 1) send();
-        c.w[c.update + c.lists++] = lists[i];
+        if (c.used() + 1 > kChangeWords) send();
+        c.w[c.used()] = lists[i];
+        c.lists++;
     }
     // (a launch has at most 2^31 workgroups)
     const int64_t most = std::max<int64_t>(1, (int64_t)0x7fff0000 / (page_bytes_ / 16384 + 1));
     for (const auto& x : moves) {
-        if (c.room() < 2 || c.moves >= most) send();
-        c.w[c.update + c.lists + 2 * c.moves] = x.first;
-        c.w[c.update + c.lists + 2 * c.moves + 1] = x.second;
+        if (c.used() + 2 > kChangeWords || c.moves >= most) send();
+        c.w[c.used()] = x.first;
+        c.w[c.used() + 1] = x.second;
         c.moves++;
     }
     send();
@@ -420,9 +431,10 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
         p.parts = 1;
     } else {
         p.tiles = by_group;
-        // The keys of a row go to several workgroups, each of which takes as many steps wherever it is: 1024 workgroups
-        // where the batch has work for them, and at least a step for each of the four waves.  A captured call is replayed
-        // when the sequences have grown: as many parts as the longest one would have.
+        // The keys of a row go to several workgroups, each of which takes as many steps wherever it is: 512 workgroups, two for
+        // each CU, where the batch has work for them (64 sequences of 32768 tokens: 1.24 ms, and 1.27 with 1024), and at least two steps
+        // for each of the four waves.  Up to four steps for each need no second launch to join them (230 tokens: 8.3 us, and
+        // 11.4 with two parts).  A captured call is replayed when the sequences have grown: as many parts as the longest one would have.
         int64_t all = 0, longest = 0;
         const int64_t most = captured ? steps_of(book_.pitch() * d.page_tokens - 1, book_.pitch() * d.page_tokens, a.window, a.sinks, step) : 0;
         for (int b = 0; b < p.batch; b++) {
@@ -433,11 +445,12 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
             longest = std::max(longest, st);
         }
         all *= (int64_t)d.kv_heads * ((group + 15) / 16);
-        int64_t chunk = std::max<int64_t>(4, (all + 1023) / 1024);
-        int64_t parts = std::max<int64_t>(1, (longest + chunk - 1) / chunk);
+        const int64_t chunk = std::max<int64_t>(8, (all + 511) / 512);
+        int64_t parts = longest <= 16 ? 1 : std::max<int64_t>(1, (longest + chunk - 1) / chunk);
         parts = std::max<int64_t>(1, std::min(parts, part_cells_ / ((int64_t)a.rows * d.heads)));
         p.chunk = (int)std::max(chunk, (longest + parts - 1) / parts);
         p.parts = (int)parts;
+        p.once = p.tiles == 1 && !book_.shares();
         p.part_o = parts_;
         p.part_ml = parts_ + part_cells_ * d.head_dim;
     }

@@ -37,6 +37,7 @@ class PageBook {
     int batch_rows() const { return words[first_at() + batch_size()]; }
     int pages_free() const { return (int)free_.size(); }
     int pages_used() const { return pages_ - (int)free_.size(); }
+    bool shares() const { return entries_ > pages_used(); }   // some page is in two lists
     int pages_of(int tokens) const { return (int)(((int64_t)tokens + page_tokens_ - 1) / page_tokens_); }
     const std::vector<int>& list(int s) const { return lists_[s]; }
 
@@ -78,6 +79,7 @@ class PageBook {
             }
             while ((int)lists_[s].size() < pages_of(len + counts[i])) {
                 lists_[s].push_back(take());
+                entries_++;
                 put(entry(s, lists_[s].size() - 1), lists_[s].back());
             }
         }
@@ -110,6 +112,7 @@ class PageBook {
             const int t = targets[i];
             lists_[t].assign(lists_[source].begin(), lists_[source].begin() + pages);
             for (int p : lists_[t]) shared_[p]++;
+            entries_ += pages;
             std::copy(lists_[t].begin(), lists_[t].end(), words.begin() + entry(t, 0));
             put(t, tokens);
         }
@@ -136,6 +139,7 @@ class PageBook {
             const int t = targets[i];
             for (int p : lists_[sources[i]]) {
                 lists_[t].push_back(take());
+                entries_++;
                 moves.push_back({p, lists_[t].back()});
                 put(entry(t, lists_[t].size() - 1), lists_[t].back());
             }
@@ -156,6 +160,7 @@ class PageBook {
             while ((int)lists_[s].size() > pages_of(keep)) {
                 const int p = lists_[s].back();
                 lists_[s].pop_back();
+                entries_--;
                 if (--shared_[p] == 0) free_.push_back(p);
             }
             put(s, keep);
@@ -211,6 +216,7 @@ class PageBook {
 
   private:
     int pages_, sequences_, page_tokens_, most_tokens_, pitch_;
+    int64_t entries_ = 0;       // of all lists
     std::vector<std::vector<int>> lists_;
     std::vector<int> shared_;   // sequences that have a page
     std::vector<int> free_;     // (a stack: the page that was freed last is taken first)

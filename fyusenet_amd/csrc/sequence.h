@@ -49,6 +49,7 @@ struct AttnParams {
     int by_token;           // a workgroup's columns: 1 sixteen tokens of a head, 0 one token and up to sixteen heads of a group
     int tiles;              // column tiles per sequence and (by_token) head or (else) key head
     // the long axis in parts
+    int once;               // no key is read by two workgroups
     int chunk;              // key steps of one part
     int parts;              // most parts of a row
     float* part_o;          // [row * heads + head][part][dim]
@@ -65,17 +66,17 @@ int attention_step(int f16, int dim);   // keys of one step of the kernel (AttnP
 
 // What the host changes of a cache in one launch.  It travels as the kernel's argument (at most 4 KB, and 256 bytes where it is
 // little: the argument's size is part of a launch's time): no memory of the host's has to outlive the call.
-// Words: {first word, number of words, words ...} ...; lists of pages that become copies of another's first entries; pages
-// that are copied.
+// Runs of words {first word, number of words, words ...} ...; single words; lists of pages that become copies of another's first
+// entries; pages that are copied.  They stand one kind behind the other in w.
 constexpr int kChangeWords = 960;
 struct CacheChange {
-    int update;             // words of the first kind in w, from 0
-    int lists;              // sequences in w behind them, whose lists become copies of the first `entries` of `source`'s
-    int moves;              // pairs {from, to} in w behind those
+    int runs;               // words that the runs take
+    int singles;            // {word, value}
+    int lists;              // sequences whose lists become copies of the first `entries` of `source`'s
+    int moves;              // {from, to}
     int source, entries;
     int w[kChangeWords];
-    int room() const { return kChangeWords - update - lists - 2 * moves; }
-    bool any() const { return update || lists || moves; }
+    int used() const { return runs + 2 * singles + lists + 2 * moves; }
 };
 struct CacheMemory {
     int* words;

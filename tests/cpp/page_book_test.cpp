@@ -81,6 +81,9 @@ struct Model {
             }
             for (int p : book.list(s)) count[p]++;
         }
+        bool shares = false;
+        for (auto& x : count) shares = shares || x.second > 1;
+        CHECK(book.shares() == shares);
         CHECK(book.pages_used() == (int)count.size() && book.pages_free() == pages - (int)count.size());
     }
     template <class F>
