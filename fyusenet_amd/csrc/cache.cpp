@@ -217,8 +217,9 @@ void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, i
     c.source = source;
     c.entries = n > 0 ? (int)book_.list(lists[0]).size() : 0;
     constexpr size_t kFew = 4;   // words of a run that go one by one: all at once then, where runs wait for each other's lengths
-    for (auto [at, end] : book_.changes())
-        while (end - at > kFew) {
+    for (auto [at, end] : book_.changes()) {
+        if (end - at <= kFew) continue;
+        while (at < end) {
             if (c.used() + 3 > kChangeWords) send();
             const int k = (int)std::min<size_t>(end - at, kChangeWords - c.used() - 2);
             c.w[c.runs] = (int)at;
@@ -227,6 +228,7 @@ void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, i
             c.runs += 2 + k;
             at += k;
         }
+    }
     for (auto [at, end] : book_.changes()) {
         if (end - at > kFew) continue;
         for (; at < end; at++) {

@@ -371,6 +371,20 @@ def test_many_sequences_and_pages():
 
 
 @pytest.mark.gpu
+def test_lists_around_a_launch():
+    """Lists of pages that end a few words in front of and behind the end of one launch's argument, or of two."""
+    k, v = values(13, "f16", (2000 * 8, 1, 8), (2000 * 8, 1, 8))
+    for pages in list(range(950, 968)) + list(range(1908, 1926)):
+        c = fa.SequenceCache(fa.STORAGE_F16, 1, 1, 1, 8, 8, 2010, 3)
+        n = pages * 8 - 3
+        c.extend([2, 0], [8, n], stream=stream())
+        c.write(0, torch.cat([v[:8], k[:n]]), torch.cat([k[:8], v[:n]]), stream=stream())
+        got_k, got_v = (torch.empty(n + 8, 1, 8, dtype=torch.float16, device="cuda") for _ in range(2))
+        c.read([0, 2], 0, got_k, got_v, stream=stream())
+        assert torch.equal(got_k, torch.cat([k[:n], v[:8]])) and torch.equal(got_v, torch.cat([v[:n], k[:8]])), pages
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("typ", ["f16", "f32"])
 def test_step_of_what_the_cache_does_not_show(typ):
     """NaN in pages behind a sequence's end, in front of its window, and in other sequences' tokens."""
