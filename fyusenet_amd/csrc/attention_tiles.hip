@@ -1,57 +1,54 @@
-// Attention of many tokens: 128, 64 or 32 queries of one head a workgroup, keys and values in tiles through shared memory.
+// Attention of many tokens: 128 or 64 queries of one head a workgroup, keys and values in tiles through shared memory.
 //
-// Each of the four waves has 32 queries as columns.  Per piece of 64 or 32 keys
+// Each of the four waves has 32 queries as columns.  Per 32 keys
 //     S^T [keys x queries]  = K Q^T          K from LDS, Q in registers for the whole run
 //     O^T [dims x queries] += V^T P^T        V^T from LDS, P^T as S^T's registers hold it
 // with the 32x32 matrix instructions.  Their result has the rows 8i + 4h + 0..3 (i = 0..3) in the lanes of half h, and the inner
 // index of the second product is ordered by that, so that the weights go from one product to the next without leaving the
-// lane.  Of a query everything, running maximum and sum too, is in two lanes.  With fewer than 128 queries two or four waves have the
-// same ones, each takes another piece of the tile's keys, and their sums are joined at the end.
+// lane.  Of a query everything, running maximum and sum too, is in two lanes.  With 64 queries two waves have the same ones, each takes
+// 32 others of the tile's keys, and their sums are joined at the end.
 //
-// The next tile's loads are under way while a tile is worked on, and go to the other half of the LDS behind it: one barrier a tile.
-// Values in 16 bits are turned in registers on the way (eight keys by four dims a thread) so that a dim's keys lie side by
-// side as the second product wants them.  Sixteen-byte pieces of rows are placed with their number xored with the row's, so
-// that the sixteen lanes that read one piece of sixteen rows find them in different banks.
+// The next tile goes from memory straight into the other half of the LDS while a tile is worked on: one barrier a tile.  Its rows
+// lie as they are in memory, their sixteen-byte pieces exchanged by a pattern of the row's number, so that the sixteen lanes that
+// read one piece of sixteen rows (keys), or pieces side by side of eight rows (values), find them in different banks.  Values in
+// 16 bits are turned by the LDS as they are read: four keys of a dim to a lane, which had four dims of a key.
 #include "attention_common.h"
 
 namespace fynhip {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr float kLag = 8.f;   // binary orders of magnitude
-typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 template <class T, int DIMS, int QW>
 struct TileShape {
     static constexpr bool F16 = std::is_same<T, _Float16>::value;
     static constexpr int KW = 4 / QW;                                            // waves with the same queries
-    static constexpr int KEYS = F16 && DIMS <= 128 && QW == 4 ? 64 : 32;         // of a wave
-    static constexpr int TILE = KEYS * KW;
+    static constexpr int TILE = 32 * KW;                                         // keys: each wave has 32 of them at once
     static constexpr int VEC = 16 / sizeof(T);
     static constexpr int PIECES = DIMS / VEC;                                    // of a row
     static constexpr int PITCH = PIECES <= 4 ? 4 : PIECES <= 8 ? 8 : PIECES <= 16 ? 16 : 32;   // ... in LDS
-    static constexpr int SPREAD = PITCH < 16 ? PITCH : 16;                       // pieces among which a row's are exchanged
-    static constexpr int SHARE = 16 / SPREAD;                                    // rows side by side in 256 bytes
-    static constexpr int LOADS = (TILE * PITCH + 255) / 256;                     // of a thread, for the keys
-    static constexpr int QUADS = DIMS / 4, GROUPS = TILE / 8;
-    static constexpr int TURNS = F16 ? (QUADS * GROUPS + 255) / 256 : LOADS;     // ... for the values
-    static constexpr int K_BYTES = TILE * PITCH * 16, V_BYTES = F16 ? DIMS * TILE * 2 : K_BYTES;
-    static constexpr int DIM_TILES = DIMS / 32, KEY_TILES = KEYS / 32;
-    static constexpr int JOIN_BYTES = KW > 1 ? 4 * DIM_TILES * 4096 : 0;         // sums of four waves
-    static constexpr int LDS = 2 * (K_BYTES + V_BYTES) > JOIN_BYTES ? 2 * (K_BYTES + V_BYTES) : JOIN_BYTES;
-    static constexpr bool FITS = LDS + 2048 <= 160 * 1024;
+    static constexpr int ALL = TILE * PITCH;                                     // pieces of a tile's keys, or values
+    static constexpr int LOADS = (ALL + 255) / 256;                              // of a lane, for the keys as for the values
+    static_assert(ALL % 256 == 0 || ALL < 256, "whole waves load");
+    static constexpr int HALF = 2 * TILE * PITCH * 16;                           // bytes of a tile: keys, then values
+    static constexpr int DIM_TILES = DIMS / 32;
+    static_assert(KW == 1 || HALF >= 2 * DIM_TILES * 4096, "sums of two waves in the place of a tile");
+    static constexpr int LDS = 2 * HALF;
+    static_assert(LDS + 2048 <= 160 * 1024, "a CU's LDS");
     static constexpr int WAVES = DIMS <= (F16 ? 128 : 64) && LDS <= 64 * 1024 ? 2 : 1;   // workgroups that share a CU (their registers)
 };
 
-__device__ __forceinline__ int row_piece(int row, int piece, int pitch, int spread, int share) { return row * pitch + (piece ^ (row / share % spread)); }
-
-// Place of the eight keys (group) of a dim.
-template <int GROUPS>
-__device__ __forceinline__ int dim_piece(int dim, int group) {
-    if (GROUPS >= 16) return dim * GROUPS + (group ^ (dim & 15));
-    if (GROUPS == 8) return dim * 8 + (group ^ ((dim >> 1 & 7) ^ (dim >> 4 & 1)));
-    return dim * 4 + (group ^ ((dim >> 2 & 3) ^ (dim >> 4 & 1)));
+// Place of a piece of a row.  (Rows side by side in 256 bytes, the banks' width, are exchanged alike.)
+template <int PITCH>
+__device__ __forceinline__ int pattern(int row) {
+    if (PITCH >= 16) return (row & 3) << 2 | (row >> 2 & 3);
+    if (PITCH == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    return row >> 2 & 3;
 }
+template <int PITCH>
+__device__ __forceinline__ int row_piece(int row, int piece) { return row * PITCH + (piece ^ pattern<PITCH>(row)); }
 
 // The larger of a lane's value and that of its other half's.
 __device__ __forceinline__ float across(float x) {
@@ -65,10 +62,11 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
     typedef TileShape<T, DIMS, QW> S;
     typedef typename Vec<T, S::VEC>::type KVec;
     constexpr bool F16 = S::F16;
-    constexpr int QUERIES = 32 * QW, HALF = S::K_BYTES + S::V_BYTES;
+    constexpr int QUERIES = 32 * QW, V_AT = S::HALF / 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, c = lane & 31, mates = wave / QW, queries = wave % QW;
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    __shared__ int odd_values[2][4];   // a wave found infinities or NaN among a tile's values
+    // (two arrays: the compiler then knows that a tile that is read is not the one that arrives)
+    __shared__ __attribute__((aligned(16))) char tile_a[S::HALF], tile_b[S::HALF];
+    __shared__ int odd_values[4];   // a wave found infinities or NaN among a tile's values
 
     // The last queries first: under a causal mask theirs are the longest runs.  Heads that share keys lie eight workgroups apart
     // where there are eight key heads, on one XCD and its L2.
@@ -131,107 +129,60 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
     };
     auto at_of = [&](int st) { return (st < a_steps ? st : b_first + st - a_steps) * S::TILE; };
 
-    u4 kreg[S::LOADS];
-    u2 vreg[F16 ? S::TURNS : 1][F16 ? 8 : 1];
-    u4 vreg32[F16 ? 1 : S::LOADS];
-    // (Pieces behind a head's last value are taken from within it: in the first product they meet queries that are zero
+    // A tile on its way: a lane's sixteen bytes go to the place that its number says, so the exchange of pieces is one of what it
+    // asks for.  (Pieces behind a head's last value are taken from within it: in the first product they meet queries that are zero
     // there, in the second they end in dims that nobody stores.)
-    const int k_piece = tid % S::PITCH, k_row = tid / S::PITCH, k_bytes = min(k_piece * 16, (p.dim - S::VEC) * (int)sizeof(T));
-    auto v_quad = [&](int i) { return (tid + i * 256) % S::QUADS; };
-    auto v_group = [&](int i) { return S::GROUPS * S::QUADS % 256 == 0 ? (tid + i * 256) / S::QUADS : min((tid + i * 256) / S::QUADS, S::GROUPS - 1); };
-    auto v_bytes = [&](int i) { return min(v_quad(i) * 8, (p.dim - 4) * 2); };
-    auto fetch = [&](int at) {
-        if (!PAGED && at + S::TILE <= most) {
-            // A thread's rows are a fixed distance from its first: one offset of 32 bits (the host has seen to that) to scalar bases.
-            const char* kb = kbase + (int64_t)at * p.k.tok * (int64_t)sizeof(T);
-            const char* vb = vbase + (int64_t)at * p.v.tok * (int64_t)sizeof(T);
-            const unsigned k_off = (unsigned)(k_row * (int)p.k.tok * (int)sizeof(T) + k_bytes);
-#pragma unroll
-            for (int i = 0; i < S::LOADS; i++) kreg[i] = *reinterpret_cast<const u4*>(kb + (int64_t)i * (256 / S::PITCH) * p.k.tok * (int64_t)sizeof(T) + k_off);
-            if constexpr (F16) {
-#pragma unroll
-                for (int i = 0; i < S::TURNS; i++) {
-                    const int g = v_group(i);
-                    const unsigned v_off = (unsigned)((g / 2 * 16 + g % 2 * 4) * (int)p.v.tok * 2 + v_bytes(i));
-#pragma unroll
-                    for (int e = 0; e < 8; e++) vreg[i][e] = *reinterpret_cast<const u2*>(vb + (int64_t)(e / 4 * 8 + e % 4) * p.v.tok * 2 + v_off);
-                }
-            } else {
-                const unsigned v_off = (unsigned)(k_row * (int)p.v.tok * (int)sizeof(T) + k_bytes);
-#pragma unroll
-                for (int i = 0; i < S::LOADS; i++) vreg32[i] = *reinterpret_cast<const u4*>(vb + (int64_t)i * (256 / S::PITCH) * p.v.tok * (int64_t)sizeof(T) + v_off);
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < S::LOADS; i++) kreg[i] = *reinterpret_cast<const u4*>(row(kbase, p.k.tok, at, k_row + i * (256 / S::PITCH), k_bytes));
-        if constexpr (F16) {
-#pragma unroll
-            for (int i = 0; i < S::TURNS; i++) {
-                const int g = v_group(i);
-#pragma unroll
-                for (int e = 0; e < 8; e++) vreg[i][e] = *reinterpret_cast<const u2*>(row(vbase, p.v.tok, at, g / 2 * 16 + e / 4 * 8 + g % 2 * 4 + e % 4, v_bytes(i)));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; i++) vreg32[i] = *reinterpret_cast<const u4*>(row(vbase, p.v.tok, at, k_row + i * (256 / S::PITCH), k_bytes));
-        }
+    const int row_bytes = p.dim * (int)sizeof(T);
+    constexpr int ROWS = 64 / S::PITCH;   // of a load
+    const int lane_row = lane / S::PITCH, lane_piece = lane % S::PITCH;
+    const unsigned k_lane = (unsigned)(lane_row * (int)p.k.tok * (int)sizeof(T)), v_lane = (unsigned)(lane_row * (int)p.v.tok * (int)sizeof(T));
+    auto arrive = [&](char* dst, const char* k, const char* v) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)k, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)v, (__attribute__((address_space(3))) void*)(dst + V_AT), 16, 0, 0);
     };
-    // `partial`: not all of the workgroup's queries see all of the tile.  Infinities and NaN among its values are left out then,
-    // and those who see them are told.
-    auto place = [&](int buf, bool partial) {
-        u4* kl = reinterpret_cast<u4*>(lds + buf * HALF);
-        u4* vl = reinterpret_cast<u4*>(lds + buf * HALF + S::K_BYTES);
+    auto fetch = [&](char* dst, int at) {
+        const bool inside = !PAGED && at + S::TILE <= most;
+        const char* kb = kbase + (int64_t)at * p.k.tok * (int64_t)sizeof(T);
+        const char* vb = vbase + (int64_t)at * p.v.tok * (int64_t)sizeof(T);
 #pragma unroll
         for (int i = 0; i < S::LOADS; i++) {
-            const int r = k_row + i * (256 / S::PITCH);
-            if (r < S::TILE) kl[row_piece(r, k_piece, S::PITCH, S::SPREAD, S::SHARE)] = kreg[i];
+            const int first = (wave * S::LOADS + i) * ROWS, bytes = min((lane_piece ^ pattern<S::PITCH>(first + lane_row)) * 16, row_bytes - 16);
+            if (S::ALL < 256 && first >= S::TILE) break;
+            char* to = dst + first * S::PITCH * 16;
+            if (inside)   // (scalar bases and 32 bits of offset: the host has seen to that)
+                arrive(to, kb + (int64_t)first * p.k.tok * (int64_t)sizeof(T) + (k_lane + bytes), vb + (int64_t)first * p.v.tok * (int64_t)sizeof(T) + (v_lane + bytes));
+            else
+                arrive(to, row(kbase, p.k.tok, at, first + lane_row, bytes), row(vbase, p.v.tok, at, first + lane_row, bytes));
         }
-        if (partial) {
-            bool found = false;
-            if constexpr (F16) {
+    };
+    // A tile that not all of the workgroup's queries see whole: infinities and NaN among its values are left out, and those who
+    // see them are told.
+    auto clean = [&](char* tile) {
+        u4* vl = reinterpret_cast<u4*>(tile + V_AT);
+        bool found = false;
 #pragma unroll
-                for (int i = 0; i < S::TURNS; i++)
+        for (int i = 0; i < S::LOADS; i++) {
+            if (S::ALL < 256 && tid >= S::ALL) break;
+            u4 x = vl[i * 256 + tid];
+            bool any_odd = false;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const unsigned x = vreg[i][e / 2][e % 2], odd = ((x & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // (an exponent of all ones carries into the sign's place)
-                        found = found || odd;
-                        vreg[i][e / 2][e % 2] = x & ~((odd << 1) - (odd >> 15));
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < S::LOADS; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const unsigned x = vreg32[i][e];
-                        const bool odd = (x & 0x7f800000u) == 0x7f800000u;
-                        found = found || odd;
-                        vreg32[i][e] = odd ? 0 : x;
-                    }
+            for (int e = 0; e < 4; e++) {
+                const unsigned y = x[e];
+                if constexpr (F16) {   // (an exponent of all ones carries into the sign's place)
+                    const unsigned odd = ((y & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                    any_odd = any_odd || odd;
+                    x[e] = y & ~((odd << 1) - (odd >> 15));
+                } else {
+                    const bool odd = (y & 0x7f800000u) == 0x7f800000u;
+                    any_odd = any_odd || odd;
+                    x[e] = odd ? 0 : y;
+                }
             }
-            found = __any(found);
-            if (lane == 0) odd_values[buf][wave] = found;
+            if (any_odd) vl[i * 256 + tid] = x;
+            found = found || any_odd;
         }
-        if constexpr (F16) {
-#pragma unroll
-            for (int i = 0; i < S::TURNS; i++) {
-                const int quad = v_quad(i), g = (tid + i * 256) / S::QUADS;
-                if (g < S::GROUPS)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        u4 t;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) t[e] = __builtin_amdgcn_perm(vreg[i][2 * e + 1][d / 2], vreg[i][2 * e][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-                        vl[dim_piece<S::GROUPS>(quad * 4 + d, g)] = t;
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; i++) {
-                const int r = k_row + i * (256 / S::PITCH);
-                if (r < S::TILE) vl[row_piece(r, k_piece, S::PITCH, S::SPREAD, S::SHARE)] = vreg32[i];
-            }
-        }
+        found = __any(found);
+        if (lane == 0) odd_values[wave] = found;
     };
     auto is_partial = [&](int at) { return !((at >= whole.lo && at + S::TILE <= whole.hi) || at + S::TILE <= whole.first); };
 
@@ -242,47 +193,67 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
         for (int r = 0; r < 16; r++) acc[d][r] = 0.f;
     float m = kNone, l = 0;   // (l: of this lane's keys only)
 
-    if (steps > 0) {
-        fetch(at_of(0));
-        place(0, is_partial(at_of(0)));
-    }
-    for (int st = 0; st < steps; st++) {
-        const int from = at_of(st), buf = st & 1, at = from + mates * S::KEYS;   // (the wave's piece)
-        __syncthreads();   // the tile is in LDS, and nobody reads the other half any more
-        if (st + 1 < steps) fetch(at_of(st + 1));
-        if ((at < any.hi && at + S::KEYS > any.lo) || at < any.first) {
-            const char* kl = lds + buf * HALF;
-            const char* vl = kl + S::K_BYTES;
-            f16v sc[S::KEY_TILES];
+    auto work = [&](char* tile, char* other, int st) {
+        const int from = at_of(st), at = from + mates * 32;   // (the wave's keys)
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // (the wave's part of the tile has arrived)
+        __syncthreads();                      // the tile is in LDS, and nobody reads the other any more
+        if (st + 1 < steps) fetch(other, at_of(st + 1));
+        __builtin_amdgcn_sched_barrier(0);
+        const bool partial = is_partial(from);
+        if (partial) {
+            clean(tile);
+            __syncthreads();
+        }
+        if ((at < any.hi && at + 32 > any.lo) || at < any.first) {
+            const char* kl = tile;
+            const char* vl = tile + V_AT;
+            f16v sc;
 #pragma unroll
-            for (int t = 0; t < S::KEY_TILES; t++)
+            for (int r = 0; r < 16; r++) sc[r] = 0.f;
+            // (All pieces of the keys are asked for before the first is needed, where there are registers for them: left to itself the
+            // compiler asks for each in front of its use, and the use waits.)
+            constexpr bool AHEAD = DIMS <= 128;
+            KVec kf[S::PIECES / 2];
 #pragma unroll
-                for (int r = 0; r < 16; r++) sc[t][r] = 0.f;
+            for (int s = 0; s < S::PIECES / 2; s++) kf[s] = *reinterpret_cast<const KVec*>(kl + 16 * row_piece<S::PITCH>(mates * 32 + c, 2 * s + half));
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < S::PIECES / 2; s++) {
+                if constexpr (F16) {
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s], q[s], sc, 0, 0, 0);
+                } else {
 #pragma unroll
-                for (int t = 0; t < S::KEY_TILES; t++) {
-                    const KVec k = *reinterpret_cast<const KVec*>(kl + 16 * row_piece(mates * S::KEYS + 32 * t + c, 2 * s + half, S::PITCH, S::SPREAD, S::SHARE));
-                    if constexpr (F16) {
-                        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], sc[t], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[s][e], sc[t], 0, 0, 0);
-                    }
+                    for (int e = 0; e < 4; e++) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[s][e], q[s][e], sc, 0, 0, 0);
                 }
             }
-            if (!((at >= all.lo && at + S::KEYS <= all.hi) || at + S::KEYS <= all.first)) {
+            if (!((at >= all.lo && at + 32 <= all.hi) || at + 32 <= all.first)) {
 #pragma unroll
-                for (int t = 0; t < S::KEY_TILES; t++)
+                for (int r = 0; r < 16; r++)
+                    if (!mine.sees(at + (r & 3) + 8 * (r >> 2) + 4 * half)) sc[r] = kNone;
+            }
+            // Dims 32 d + c, keys 4 half .. + 3 of the sixteen t, and those 8 further on.  A lane names what it has before they are
+            // turned: key lane / 4 % 4 of the four, and the dims from 16 (c / 16) + 4 (lane % 4) on.
+            auto value = [&](int t, int d) {
+                h8 v;
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (!mine.sees(at + 32 * t + (r & 3) + 8 * (r >> 2) + 4 * half)) sc[t][r] = kNone;
+                for (int e = 0; e < 2; e++) {
+                    const int key = mates * 32 + 16 * t + 8 * e + 4 * half + (lane >> 2 & 3), dim = 32 * d + 16 * (c >> 4) + 4 * (lane & 3);
+                    const h4 four = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s4*)(vl + 16 * row_piece<S::PITCH>(key, dim / 8) + dim % 8 * 2)));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[4 * e + i] = four[i];
+                }
+                return v;
+            };
+            h8 vf[F16 ? S::DIM_TILES : 1];
+            if constexpr (F16) {
+#pragma unroll
+                for (int d = 0; d < S::DIM_TILES; d++) vf[d] = value(0, d);
+                if (AHEAD) __builtin_amdgcn_sched_barrier(0);
             }
             float top = kNone;
 #pragma unroll
-            for (int t = 0; t < S::KEY_TILES; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) top = fmaxf(top, sc[t][r]);
+            for (int r = 0; r < 16; r++) top = fmaxf(top, sc[r]);
             top = across(top) * scale;
             // The sums are relative to a maximum that may be the true one's 2^-8 (with weights up to 2^14 then): it follows where a
             // query is further off, which after the first tiles is seldom.
@@ -299,42 +270,43 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
             // They are rounded to 16 bits for the second product, and it is the rounded ones that are summed up.
             const float base = m == kNone ? 0.f : m - 6.f;
 #pragma unroll
-            for (int t = 0; t < S::KEY_TILES; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], scale, -base));
+            for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -base));
             if constexpr (F16) {
-                h8 w[2 * S::KEY_TILES];
+                h8 w[2];
 #pragma unroll
-                for (int t = 0; t < 2 * S::KEY_TILES; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        const h2 two = {(_Float16)sc[t / 2][t % 2 * 8 + e], (_Float16)sc[t / 2][t % 2 * 8 + e + 1]};
+                        const h2 two = {(_Float16)sc[t * 8 + e], (_Float16)sc[t * 8 + e + 1]};
                         l = __builtin_amdgcn_fdot2(two, h2{(_Float16)1, (_Float16)1}, l, false);
                         w[t][e] = two[0];
                         w[t][e + 1] = two[1];
                     }
 #pragma unroll
-                for (int t = 0; t < 2 * S::KEY_TILES; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int d = 0; d < S::DIM_TILES; d++) {
-                        const h8 v = *reinterpret_cast<const h8*>(vl + 16 * dim_piece<S::GROUPS>(32 * d + c, mates * (S::KEYS / 8) + 2 * t + half));
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[t], acc[d], 0, 0, 0);
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], w[t], acc[d], 0, 0, 0);
+                        if (t == 0) {
+                            vf[d] = value(1, d);
+                            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; r++) l += sc[0][r];
+                for (int r = 0; r < 16; r++) l += sc[r];
 #pragma unroll
                 for (int r = 0; r < 16; r++)
 #pragma unroll
                     for (int d = 0; d < S::DIM_TILES; d++) {
-                        const int key = mates * S::KEYS + (r & 3) + 8 * (r >> 2) + 4 * half, dim = 32 * d + c;
-                        const float v = *reinterpret_cast<const float*>(vl + 16 * row_piece(key, dim / 4, S::PITCH, S::SPREAD, S::SHARE) + dim % 4 * 4);
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[0][r], acc[d], 0, 0, 0);
+                        const int key = mates * 32 + (r & 3) + 8 * (r >> 2) + 4 * half, dim = 32 * d + c;
+                        const float v = *reinterpret_cast<const float*>(vl + 16 * row_piece<S::PITCH>(key, dim / 4) + dim % 4 * 4);
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[r], acc[d], 0, 0, 0);
                     }
             }
             // Values that were left out: whoever sees them has them in the result (a weight is never negative).
-            if (is_partial(from) && (odd_values[buf][0] | odd_values[buf][1] | odd_values[buf][2] | odd_values[buf][3])) {
-                for (int key = 0; key < S::KEYS; key++) {
+            if (partial && (odd_values[0] | odd_values[1] | odd_values[2] | odd_values[3])) {
+                for (int key = 0; key < 32; key++) {
                     const T* v = reinterpret_cast<const T*>(row(vbase, p.v.tok, at, key, 0));
                     const bool sees = mine.sees(at + key);
                     int h4 = 4 * half;
@@ -350,7 +322,11 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
                 }
             }
         }
-        if (st + 1 < steps) place(buf ^ 1, is_partial(at_of(st + 1)));
+    };
+    if (steps > 0) fetch(tile_a, at_of(0));
+    for (int st = 0; st < steps; st += 2) {
+        work(tile_a, tile_b, st);
+        if (st + 1 < steps) work(tile_b, tile_a, st + 1);
     }
 
     l += __shfl_xor(l, 32);
@@ -368,11 +344,11 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
         for (int k = 0; k < S::KW; k++) total += top == kNone ? 0.f : totals[k * QW + queries][c] * __builtin_amdgcn_exp2f(tops[k * QW + queries][c] - top);
         const float f = top == kNone ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        float* sums = reinterpret_cast<float*>(lds);
+        auto sums = [&](int w, int d, int r) -> float& { return reinterpret_cast<float*>(w < 2 ? tile_a : tile_b)[(((w & 1) * S::DIM_TILES + d) * 16 + r) * 64 + lane]; };
 #pragma unroll
         for (int d = 0; d < S::DIM_TILES; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) sums[((wave * S::DIM_TILES + d) * 16 + r) * 64 + lane] = acc[d][r] * f;
+            for (int r = 0; r < 16; r++) sums(wave, d, r) = acc[d][r] * f;
         __syncthreads();
 #pragma unroll
         for (int d = 0; d < S::DIM_TILES; d++)
@@ -381,7 +357,7 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
                 for (int r = 0; r < 16; r++) {
                     float sum = 0;
 #pragma unroll
-                    for (int k = 0; k < S::KW; k++) sum += sums[(((k * QW + queries) * S::DIM_TILES + d) * 16 + r) * 64 + lane];
+                    for (int k = 0; k < S::KW; k++) sum += sums(k * QW + queries, d, r);
                     acc[d][r] = sum;
                 }
         l = total;
@@ -405,23 +381,17 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 }
 
 template <class T, int DIMS, int QW>
-static bool launch_tiles(const AttnParams& p, unsigned blocks, hipStream_t s) {
-    if constexpr (TileShape<T, DIMS, QW>::FITS) {
-        if (p.paged) hipLaunchKernelGGL((attend_tiles<T, DIMS, true, QW>), dim3(blocks), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((attend_tiles<T, DIMS, false, QW>), dim3(blocks), dim3(256), 0, s, p);
-        return true;
-    }
-    return false;
+static void launch_tiles(const AttnParams& p, unsigned blocks, hipStream_t s) {
+    if (p.paged) hipLaunchKernelGGL((attend_tiles<T, DIMS, true, QW>), dim3(blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attend_tiles<T, DIMS, false, QW>), dim3(blocks), dim3(256), 0, s, p);
 }
 
 #if FYN_ATTN_HALF
 typedef _Float16 Stored;
 #define FYN_ATTN_NAME launch_tiles_f16
-#define FYN_ATTN_FITS tiles_fit_f16
 #else
 typedef float Stored;
 #define FYN_ATTN_NAME launch_tiles_f32
-#define FYN_ATTN_FITS tiles_fit_f32
 #endif
 
 template <int QW>
@@ -429,34 +399,18 @@ static int launch_class(const AttnParams& p, hipStream_t s) {
     const int64_t blocks = ((int64_t)p.batch * p.heads + 7) / 8 * 8 * p.tiles;
     if (blocks <= 0) return 0;
     if (blocks > 0x7fffffff) return -1;
-    bool done = false;
-    if (p.dim <= 32) done = launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 64) done = launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 96) done = launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 128) done = launch_tiles<Stored, 128, QW>(p, (unsigned)blocks, s);
+    if (p.dim <= 32) launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 64) launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 96) launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 128) launch_tiles<Stored, 128, QW>(p, (unsigned)blocks, s);
 #if FYN_ATTN_HALF
-    else done = launch_tiles<Stored, 256, QW>(p, (unsigned)blocks, s);
-#endif
-    return done && hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
-int FYN_ATTN_NAME(const AttnParams& p, hipStream_t s) {
-    return p.tiled == 128 ? launch_class<4>(p, s) : p.tiled == 64 ? launch_class<2>(p, s) : launch_class<1>(p, s);
-}
-
-template <int QW>
-static bool fits(int dim) {
-    if (dim <= 32) return TileShape<Stored, 32, QW>::FITS;
-    if (dim <= 64) return TileShape<Stored, 64, QW>::FITS;
-    if (dim <= 96) return TileShape<Stored, 96, QW>::FITS;
-    if (dim <= 128) return TileShape<Stored, 128, QW>::FITS;
-#if FYN_ATTN_HALF
-    return TileShape<Stored, 256, QW>::FITS;
+    else launch_tiles<Stored, 256, QW>(p, (unsigned)blocks, s);
 #else
-    return false;   // (queries and sums of 32 bits: more registers than a wave has)
+    else return -1;   // (queries and sums of 32 bits: more registers than a wave has)
 #endif
+    return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-bool FYN_ATTN_FITS(int dim, int queries) { return queries == 128 ? fits<4>(dim) : queries == 64 ? fits<2>(dim) : fits<1>(dim); }
+int FYN_ATTN_NAME(const AttnParams& p, hipStream_t s) { return p.tiled == 128 ? launch_class<4>(p, s) : launch_class<2>(p, s); }
 
 }  // namespace fynhip

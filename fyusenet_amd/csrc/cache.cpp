@@ -47,16 +47,18 @@ static void check_storage(int storage) {
     if (storage != FYN_STORAGE_F32 && storage != FYN_STORAGE_F16) fail(FYN_ERR_INVALID, "unknown storage type %d", storage);
 }
 
-// How many tokens of a head a workgroup of the kernel with tiles in shared memory gets; 0: the call is not for it.
-static int tiled(const AttnParams& p) {
+// How many of the `tokens` tokens of a head a workgroup of the kernel with tiles in shared memory gets; 0: the call is not for it.
+static int tiled(const AttnParams& p, int tokens) {
+    if (p.dim > 128 && !p.f16) return 0;
     if (!p.paged && std::max(p.k.tok, p.v.tok) * (p.f16 ? 2 : 4) > (1 << 24)) return 0;      // (32 bits of offset within a tile)
-    // Large workgroups read keys and values the fewest times, small ones are more: 128 queries where that gives workgroups
-    // for one and a half of the chip's CUs (16 heads of 4096 tokens: 108 us, against 150 with 64), 64 where it gives them for
-    // half of them (8 heads of 2048 tokens, two sequences: 52 us, against 61 with 128 and 121 without tiles).
+    // Large workgroups read keys and values the fewest times, small ones are more: 128 queries where that gives two workgroups
+    // for each CU (32 heads, 4 ragged prompts of up to 2001 tokens, window 512, fp16: 115 us, against 134 with 64; half as many
+    // workgroups, 8 heads of 2048 tokens, two sequences: 58 us, against 39 with 64), 64 where it gives them for three quarters of the
+    // CUs (12 heads of 197 tokens, four sequences: 8.0 us, against 10.7 without tiles; 8 heads of 1024 tokens, fp32, which is half
+    // of the CUs: 99 us, against 64).
     const int64_t units = (int64_t)p.batch * p.heads;
-    auto fit = p.f16 ? tiles_fit_f16 : tiles_fit_f32;
-    if (units * ((p.tokens + 127) / 128) >= 384 && fit(p.dim, 128)) return 128;
-    if (units * ((p.tokens + 63) / 64) >= 128 && fit(p.dim, 64)) return 64;
+    if (units * ((tokens + 127) / 128) >= 512) return 128;
+    if (units * ((tokens + 63) / 64) >= 192) return 64;
     return 0;
 }
 
@@ -88,7 +90,7 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     p.by_token = 1;
     p.chunk = 0x7fffffff;
     p.parts = 1;
-    p.tiled = tiled(p);
+    p.tiled = tiled(p, a.tokens);
     const int columns = p.tiled ? p.tiled : 16;
     p.tiles = (a.tokens + columns - 1) / columns;
     return true;
@@ -428,7 +430,9 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
     const int by_group = most_new * ((group + 15) / 16), by_token = (most_new + 15) / 16 * group;
     if (by_token < by_group) {
         p.by_token = 1;
-        p.tiles = (most_new + 15) / 16;
+        p.tiled = tiled(p, most_new);
+        const int columns = p.tiled ? p.tiled : 16;
+        p.tiles = (most_new + columns - 1) / columns;
         p.chunk = 0x7fffffff;
         p.parts = 1;
     } else {

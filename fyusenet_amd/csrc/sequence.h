@@ -45,7 +45,7 @@ struct AttnParams {
     int causal, window, sinks;
     float scale_log2;       // softmax scale times log2(e)
     // rows of one launch
-    int tiled;              // attention_tiles.hip: tokens of a head that a workgroup has (128, 64 or 32), or 0: attention.hip
+    int tiled;              // attention_tiles.hip: tokens of a head that a workgroup has (128 or 64), or 0: attention.hip
     int by_token;           // a workgroup's columns: 1 sixteen tokens of a head, 0 one token and up to sixteen heads of a group
     int tiles;              // column tiles per sequence and (by_token) head or (else) key head
     // the long axis in parts
@@ -59,9 +59,7 @@ struct AttnParams {
 // 0, or -1 where the launch failed.
 int launch_attention(const AttnParams& p, hipStream_t s);
 int launch_tiles_f16(const AttnParams& p, hipStream_t s);   // (called by it)
-int launch_tiles_f32(const AttnParams& p, hipStream_t s);
-bool tiles_fit_f16(int dim, int queries);                   // whether there is such a kernel: its tiles fit into the LDS
-bool tiles_fit_f32(int dim, int queries);
+int launch_tiles_f32(const AttnParams& p, hipStream_t s);   // ... up to 128 dims
 int attention_step(int f16, int dim);   // keys of one step of the kernel (AttnParams::chunk counts them)
 
 // What the host changes of a cache in one launch.  It travels as the kernel's argument (at most 4 KB, and 256 bytes where it is

@@ -297,6 +297,19 @@ def test_several_tokens_over_the_cache(typ, heads, kv, dim, page):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim,page,counts", [(16, 4, 64, 8, [260, 3, 257, 100]), (16, 2, 128, 32, [200, 65, 190, 129]), (32, 4, 80, 16, [300, 1, 64, 270, 128, 129])])
+def test_pieces_of_prompts_over_the_cache(typ, heads, kv, dim, page, counts):
+    """Pieces with enough tokens for tiles, one behind the other."""
+    n = len(counts)
+    p = Pair(typ, heads, kv, dim, page, 40 * n * 16 // page + 200, n)
+    p.extend(list(range(n)), [17 + i for i in range(n)], window=0, sinks=0)
+    p.extend(list(range(n))[::-1], counts, window=0, sinks=0)
+    p.extend(list(range(n)), counts, window=90, sinks=20)
+    p.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["f16", "f32"])
 def test_pages_and_attention_together(typ):
     """What a service does with a cache, step by step: prompts, branches, steps, copies, sequences that are cut and end,
     compaction; every step's attention and all that the cache holds are looked at."""
