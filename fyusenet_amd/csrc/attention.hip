@@ -432,7 +432,7 @@ int launch_attention(const AttnParams& p, hipStream_t s) {
     const int64_t across = p.by_token ? p.heads : p.kv_heads;
     const int64_t blocks = (across * p.parts + 7) / 8 * 8 * (int64_t)p.tiles * p.batch;
     if (blocks <= 0) return 0;
-    if (blocks > 0x7fffffff) return -1;
+    if (blocks > 0x7fffffff) return -2;
 #define FYN_ATTN(T, D) launch_steps<T, D>(p, (unsigned)blocks, s)
     if (p.f16) {
         if (p.dim <= 32) FYN_ATTN(_Float16, 32);

@@ -398,7 +398,7 @@ template <int QW>
 static int launch_class(const AttnParams& p, hipStream_t s) {
     const int64_t blocks = ((int64_t)p.batch * p.heads + 7) / 8 * 8 * p.tiles;
     if (blocks <= 0) return 0;
-    if (blocks > 0x7fffffff) return -1;
+    if (blocks > 0x7fffffff) return -2;
     if (p.dim <= 32) launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
     else if (p.dim <= 64) launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
     else if (p.dim <= 96) launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);

@@ -35,7 +35,7 @@ static float scale_log2(float scale, int dim) { return (scale == 0.f ? 1.f / std
 
 static void check_sight(int window, int sinks, float scale) {
     if (window < 0 || sinks < 0) fail(FYN_ERR_INVALID, "attention: window %d and sinks %d must not be negative", window, sinks);
-    if (!std::isfinite(scale)) fail(FYN_ERR_INVALID, "attention: the scale is not finite");
+    if (!std::isfinite(scale * 1.44269504f)) fail(FYN_ERR_INVALID, "attention: the scale is not finite, or too large");
 }
 
 static void check_heads(int heads, int kv_heads, int dim) {
@@ -96,12 +96,18 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     return true;
 }
 
+void run_attention(const AttnParams& p, hipStream_t s) {
+    const int rc = launch_attention(p, s);
+    if (rc == -2) fail(FYN_ERR_INVALID, "attention: more heads and tokens than one launch takes");
+    if (rc != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
+}
+
 void attention(const fyn_attention_desc& a, hipStream_t s) {
     AttnParams p;
     int device;
     if (!attention_params(a, p, device)) return;
     OnDevice on(device);
-    if (launch_attention(p, s) != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
+    run_attention(p, s);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -169,6 +175,8 @@ static bool capturing(hipStream_t s) {
 
 void Cache::join_streams(hipStream_t s) {
     if (used_ && last_ != s) {
+        // (its work from before the capture could not be waited for without becoming part of the capture)
+        if (capturing(last_)) fail(FYN_ERR_STATE, "cache: the stream that it was used on last is being captured");
         // (a stream that is gone cannot be asked: everything on the device then)
         if (hipEventRecord(between_, last_) == hipSuccess) {
             FYN_HIP(hipStreamWaitEvent(s, between_, 0));
@@ -198,10 +206,13 @@ void Cache::order(hipStream_t s) {
     enter(s);
 }
 
-void Cache::expect(int rows, hipStream_t s) {
+std::vector<int> Cache::expect(int rows, hipStream_t s) {
     std::lock_guard<std::mutex> lock(mu_);
     if (rows != book_.batch_rows()) fail(FYN_ERR_INVALID, "cache: the batch has %d new tokens, the layer %d positions", book_.batch_rows(), rows);
+    OnDevice on(device);
     enter(s);
+    const int* first = book_.words.data() + book_.first_at();
+    return std::vector<int>(first, first + book_.batch_size() + 1);
 }
 
 // What the book has changed, on the device: words, lists that are copies of another's, pages that are copied; in as few launches
@@ -460,7 +471,7 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
         p.part_o = parts_;
         p.part_ml = parts_ + part_cells_ * d.head_dim;
     }
-    if (launch_attention(p, s) != 0) fail(FYN_ERR_DEVICE, "cache: launch failed");
+    run_attention(p, s);
 }
 
 }  // namespace fynhip

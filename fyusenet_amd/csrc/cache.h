@@ -23,7 +23,8 @@ class Cache : public std::enable_shared_from_this<Cache> {
     void compact(int* used, hipStream_t s);
     void lengths(int n, const int* seqs, int* tokens);
     void pages(int* used, int* free);
-    void expect(int rows, hipStream_t s);   // a pass over the batch follows on this stream, for so many new tokens
+    // A pass over the batch follows on this stream, for so many new tokens.  -> the rows at which its sequences begin
+    std::vector<int> expect(int rows, hipStream_t s);
     void order(hipStream_t s);   // what has been queued on the stream that the cache was used on last comes before what follows on this one
 
     const int device;
@@ -54,6 +55,7 @@ class Cache : public std::enable_shared_from_this<Cache> {
 
 // Attention over dense tensors.
 void attention(const fyn_attention_desc& a, hipStream_t s);
+void run_attention(const AttnParams& p, hipStream_t s);
 bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device);   // checked; false: nothing to do
 
 // The current device for the length of a call.

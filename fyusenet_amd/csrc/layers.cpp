@@ -688,10 +688,16 @@ class AttentionLayer : public Layer {
         w.erase(std::remove(w.begin(), w.end(), this), w.end());
         if (cache) w.push_back(this);
     }
-    void before_pass(hipStream_t s) override { cache->expect(oh * ow, s); }
+    void before_pass(hipStream_t s) override {
+        // (a captured pass is for a batch of as many sequences with as many new tokens each)
+        std::vector<int> now = cache->expect(oh * ow, s);
+        if (now == first) return;
+        first = std::move(now);
+        net->weights_changed();
+    }
     void forward(hipStream_t s) override {
         if (!cache) {
-            if (launch_attention(p, s) != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
+            run_attention(p, s);
             return;
         }
         fyn_attend_desc a{};
@@ -723,6 +729,7 @@ class AttentionLayer : public Layer {
     AttnParams p{};
     std::shared_ptr<Cache> cache;
     int cache_layer = 0;
+    std::vector<int> first;
 };
 
 class UploadLayer : public Layer {

@@ -5,6 +5,7 @@
 #pragma once
 #include <algorithm>
 #include <cstdint>
+#include <exception>
 #include <string>
 #include <utility>
 #include <vector>
@@ -13,7 +14,9 @@ namespace fynhip {
 
 class PageBook {
   public:
-    struct Refused {
+    struct Refused : public std::exception {
+        Refused(bool f, std::string w) : full(f), why(std::move(w)) {}
+        const char* what() const noexcept override { return why.c_str(); }
         bool full;   // no pages left (else: an argument is wrong)
         std::string why;
     };
@@ -223,7 +226,7 @@ class PageBook {
     std::vector<char> mark_;
     std::vector<std::pair<size_t, size_t>> changes_;
 
-    [[noreturn]] static void refuse(bool full, const std::string& why) { throw Refused{full, why}; }
+    [[noreturn]] static void refuse(bool full, const std::string& why) { throw Refused(full, why); }
     void empty(int s) {
         if (words[s] != 0) refuse(false, "sequence " + std::to_string(s) + " has tokens already");
     }

@@ -56,7 +56,7 @@ struct AttnParams {
     float* part_ml;         // ... [2]: maximum and sum
 };
 
-// 0, or -1 where the launch failed.
+// 0, -1 where the launch failed, -2 where it would have more workgroups than there can be.
 int launch_attention(const AttnParams& p, hipStream_t s);
 int launch_tiles_f16(const AttnParams& p, hipStream_t s);   // (called by it)
 int launch_tiles_f32(const AttnParams& p, hipStream_t s);   // ... up to 128 dims

@@ -174,6 +174,44 @@ def test_network_over_a_cache(storage, graph):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("storage", STORAGES)
+def test_captured_pass_follows_the_batch(storage):
+    """The same network, captured, over batches of the same number of tokens that are divided differently; bound before it is set up."""
+    heads, kv, dim, rows = 4, 2, 32, 6
+    cache = fa.SequenceCache(storage, 1, heads, kv, dim, 8, 60, 6)
+
+    class Net(fa.NeuralNetwork):
+        def buildLayers(self, factory):
+            builder(heads, kv, dim, rows, 1).causal().push(factory)
+
+        def connectLayers(self, layers, bm):
+            layers[1].bindCache(cache)
+
+    net = Net(storage)
+    net.setup()
+    net.useGraph(True)
+    typ = np.float16 if storage == fa.STORAGE_F16 else np.float32
+    rng = np.random.default_rng(6)
+    past = {s: [] for s in range(6)}
+    for who, counts in (([0, 1, 2, 3, 4, 5], [1] * 6), ([0, 1, 2, 3, 4, 5], [1] * 6), ([3, 1], [2, 4]), ([2], [6]), ([0, 5, 4], [3, 0, 3]), ([0, 1, 2, 3, 4, 5], [1] * 6)):
+        ins = [rng.standard_normal((n * dim, 1, rows)).astype(typ).astype(np.float32) for n in (heads, kv, kv)]
+        for port, x in enumerate(ins):
+            net.layers[1].setInput(x, port)
+        cache.extend(who, counts)
+        net.forward()
+        net.finish()
+        got = tokens(net.layers[1].copyResult(), heads, storage)[0]
+        q, k, v = (tokens(x, n, storage)[0] for x, n in zip(ins, (heads, kv, kv)))
+        at = 0
+        for s, m in zip(who, counts):
+            past[s].append((k[at:at + m], v[at:at + m]))
+            ks, vs = (torch.cat([x[i] for x in past[s]]) for i in (0, 1))
+            close(got[at:at + m], *reference(q[at:at + m], ks, vs, ks.shape[0] - m))
+            at += m
+    net.cleanup()
+
+
+@pytest.mark.gpu
 def test_attention_layer_in_a_network_with_buffer_reuse():
     """The same block with and without shared buffers, eager and from the captured graph: the same bits."""
     x = np.random.default_rng(8).standard_normal((Block.CHANNELS, 12, 31)).astype(np.float32)

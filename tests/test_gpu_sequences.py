@@ -484,6 +484,38 @@ def test_other_streams():
     close(out, *reference(q, k, v, 19999))
 
 
+@pytest.mark.gpu
+def test_two_threads():
+    """Two caches, each driven by a thread of its own, and attention over tensors in both."""
+    import threading
+    wrong = []
+
+    def work(seed):
+        try:
+            own = torch.cuda.Stream()
+            with torch.cuda.stream(own):
+                p = Pair("f16", 4, 2, 64, 16, 200, 3)
+                p.seed = 1000 * seed
+                for i in range(6):
+                    p.extend([0, 2, 1], [1 + 7 * i * seed, 3, 20], window=0, sinks=0)
+                    if i == 2:
+                        p.cache.compact(stream=stream())
+                q, k, v = values(seed, "f16", (2, 300, 8, 64), (2, 300, 4, 64), (2, 300, 4, 64))
+                out = torch.empty_like(q)
+                fa.attention(q, k, v, out, stream=stream())
+                close(out[1], *reference(q[1], k[1], v[1], 0))
+                p.check()
+        except BaseException as e:   # noqa: BLE001 -- told to the test's own thread
+            wrong.append(e)
+
+    both = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    for t in both:
+        t.start()
+    for t in both:
+        t.join()
+    assert not wrong, wrong
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # refusals (no GPU is asked before an argument is)
 # ---------------------------------------------------------------------------------------------------------------------
@@ -499,7 +531,7 @@ def _attention_desc(**kw):
 @pytest.mark.parametrize("wrong,code", [
     ({"struct_size": 4}, capi.ERR_INVALID), ({"storage": 2}, capi.ERR_INVALID), ({"heads": 3}, capi.ERR_INVALID), ({"kv_heads": 0}, capi.ERR_INVALID),
     ({"head_dim": 12}, capi.ERR_UNSUPPORTED), ({"head_dim": 264}, capi.ERR_UNSUPPORTED), ({"head_dim": 0}, capi.ERR_UNSUPPORTED),
-    ({"window": -1}, capi.ERR_INVALID), ({"sinks": -1}, capi.ERR_INVALID), ({"scale": math.nan}, capi.ERR_INVALID),
+    ({"window": -1}, capi.ERR_INVALID), ({"sinks": -1}, capi.ERR_INVALID), ({"scale": math.nan}, capi.ERR_INVALID), ({"scale": 3e38}, capi.ERR_INVALID),
     ({"batch": -1}, capi.ERR_INVALID), ({"tokens": -1}, capi.ERR_INVALID), ({"batch": 1 << 20, "tokens": 1 << 20}, capi.ERR_INVALID), ({}, capi.ERR_INVALID),
 ], ids=lambda x: "_".join("%s%s" % i for i in x.items()) or "null" if isinstance(x, dict) else "")
 def test_attention_refuses(wrong, code):
