@@ -64,40 +64,52 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
 
     // Which part of which columns.  Workgroups that read the same keys for different sequences (branches of one sequence
     // share pages) or columns lie eight apart, which is on one XCD and its L2, one behind the other.
+    constexpr bool BRANCHES = PAGED && !BY_TOKEN && !ONCE;   // some tokens may be those of all sequences (AttnParams::common)
     const int group = p.heads / p.kv_heads, across = BY_TOKEN ? p.heads : p.kv_heads;
-    const int columns = p.tiles * p.batch;
-    const int id = blockIdx.x, x = (id / (8 * columns)) * 8 + id % 8, col_tile = id / 8 % columns;
-    if (x >= across * p.parts) return;
-    const int part = x / across, who = x % across, b = col_tile / p.tiles, tile = col_tile % p.tiles;
+    const int common_blocks = BRANCHES && p.common ? (across * p.common_parts + 7) / 8 * 8 * p.common_tiles : 0;
+    const bool together = BRANCHES && (int)blockIdx.x < common_blocks;
+    const int columns = together ? p.common_tiles : p.tiles * p.batch, parts = together ? p.common_parts : p.parts - (BRANCHES ? p.common_parts : 0);
+    const int id = (int)blockIdx.x - (together ? 0 : common_blocks), x = (id / (8 * columns)) * 8 + id % 8, col_tile = id / 8 % columns;
+    if (x >= across * parts) return;
+    const int part = x / across, who = x % across, b = together ? 0 : col_tile / p.tiles, tile = together ? 0 : col_tile % p.tiles;
     const int kv_head = BY_TOKEN ? who / group : who;
 
     const Batched in = batched<PAGED>(p, b);
     const int len = in.len, count = in.count, row0 = in.row0, seq = in.seq, pos0 = in.pos0;
     const int token_tile = BY_TOKEN ? tile : tile / ((group + 15) / 16);
-    const int tok = BY_TOKEN ? token_tile * 16 + c : token_tile;
     if ((BY_TOKEN ? token_tile * 16 : token_tile) >= count) return;
-    const int in_group = BY_TOKEN ? 0 : tile % ((group + 15) / 16) * 16 + c;
-    const int head = BY_TOKEN ? who : kv_head * group + in_group;
-    const bool valid = BY_TOKEN ? tok < count : in_group < group;
+    // a column's row of the queries (from row0 on) and its head; whether there is such a column
+    const int first_head = BY_TOKEN ? 0 : tile % ((group + 15) / 16) * 16;
+    auto row_of = [&](int col) { return together ? (col_tile * 16 + col) / group : BY_TOKEN ? token_tile * 16 + col : token_tile; };
+    auto head_of = [&](int col) { return together ? kv_head * group + (col_tile * 16 + col) % group : BY_TOKEN ? who : kv_head * group + first_head + col; };
+    auto exists = [&](int col) { return together ? col_tile * 16 + col < min(p.batch, p.tokens) * group : BY_TOKEN ? token_tile * 16 + col < count : first_head + col < group; };
+    const int tok = row_of(c), head = head_of(c);
+    const bool valid = exists(c);
     const bool inside = PAGED || pos0 + tok < len;   // (a padded row sees nothing)
 
     // what the columns see, one by one and together
-    Sight mine = sight_of(pos0 + tok, len, p.causal, p.window, p.sinks);
-    if (!valid || !inside) mine.lo = mine.hi = mine.first = 0;
-    const int tok_a = BY_TOKEN ? token_tile * 16 : tok, tok_b = BY_TOKEN ? min(tok_a + 15, (PAGED ? count : min(count, len)) - 1) : tok;
-    Sight any = sight_of(pos0 + tok_a, len, p.causal, p.window, p.sinks), all = any;
-    if (tok_b < tok_a || (!PAGED && pos0 + tok_a >= len)) {
-        any.lo = any.hi = any.first = 0;
-        all = any;
-    } else if (BY_TOKEN) {
-        const Sight last = sight_of(pos0 + tok_b, len, p.causal, p.window, p.sinks);
-        any.hi = last.hi; any.first = last.first;
-        all.lo = last.lo;
+    Sight mine, any, all;
+    if (together) {
+        mine = any = all = Sight{0, p.common, 0};
+    } else {
+        mine = sight_of(pos0 + tok, len, p.causal, p.window, p.sinks);
+        const int tok_a = BY_TOKEN ? token_tile * 16 : token_tile, tok_b = BY_TOKEN ? min(tok_a + 15, (PAGED ? count : min(count, len)) - 1) : token_tile;
+        any = all = sight_of(pos0 + tok_a, len, p.causal, p.window, p.sinks);
+        if (tok_b < tok_a || (!PAGED && pos0 + tok_a >= len)) {
+            any.lo = any.hi = any.first = 0;
+            all = any;
+        } else if (BY_TOKEN) {
+            const Sight last = sight_of(pos0 + tok_b, len, p.causal, p.window, p.sinks);
+            any.hi = last.hi; any.first = last.first;
+            all.lo = last.lo;
+        }
+        if (BRANCHES && p.common) mine.lo = any.lo = all.lo = p.common;
     }
+    if (!valid || !inside) mine.lo = mine.hi = mine.first = 0;
     const int a_steps = (any.first + S::STEP - 1) / S::STEP, b_first = max(any.lo / S::STEP, a_steps);
     const int b_steps = max(0, (any.hi + S::STEP - 1) / S::STEP - b_first), steps = a_steps + b_steps;
     // (equal parts for every row, so that those of long and short sequences take equally long)
-    const int chunk = max(p.chunk, (steps + p.parts - 1) / p.parts), begin = part * chunk, end = min(steps, begin + chunk);
+    const int chunk = max(together ? p.common_chunk : p.chunk, (steps + parts - 1) / parts), begin = part * chunk, end = min(steps, begin + chunk);
     if (begin > 0 && begin >= end) return;
     const int most = max(any.hi, any.first);   // positions from here on are not read
 
@@ -337,9 +349,8 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     __syncthreads();
     // (sixteen threads for a column)
     const int col = threadIdx.x >> 4, sub = threadIdx.x & 15;
-    const int o_tok = BY_TOKEN ? token_tile * 16 + col : token_tile;
-    const int o_in = BY_TOKEN ? 0 : in_group - c + col, o_head = BY_TOKEN ? who : kv_head * group + o_in;
-    if (BY_TOKEN ? o_tok >= count : o_in >= group) return;
+    const int o_tok = row_of(col), o_head = head_of(col);
+    if (!exists(col)) return;
     float mm = kNone;
     for (int w = 0; w < 4; w++) mm = fmaxf(mm, tops[w][col]);
     const float base = mm == kNone ? 0.f : mm;
@@ -348,12 +359,12 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
         f[w] = __builtin_amdgcn_exp2f(tops[w][col] - base);
         total += totals[w][col] * f[w];
     }
-    const bool only = steps <= chunk;   // the row has one part
+    const bool only = steps <= chunk && !(BRANCHES && p.common);   // the row has one part
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const bool zero = !PAGED && o_tok >= len;   // (a padded row: its column took part in steps that all others see whole)
     const int64_t r_out = (int64_t)row0 + o_tok;
     T* dst = reinterpret_cast<T*>(p.out.p) + (PAGED ? 0 : b * p.out.seq) + r_out * p.out.tok + (int64_t)o_head * p.out.head;
-    const int64_t cell = ((PAGED ? r_out : (int64_t)b * p.tokens + r_out) * p.heads + o_head) * p.parts + part;
+    const int64_t cell = ((PAGED ? r_out : (int64_t)b * p.tokens + r_out) * p.heads + o_head) * p.parts + (BRANCHES && !together ? p.common_parts : 0) + part;
     for (int d = sub * 4; d < p.dim; d += 64) {
         f4 o = {0, 0, 0, 0};
 #pragma unroll
@@ -391,12 +402,13 @@ __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
     }
     const int len = p.words.len[p.words.batch[lo]], pos = len - (p.words.first[lo + 1] - (int)row);
     // the parts that attend_steps made
-    const Sight see = sight_of(pos, len, p.causal, p.window, p.sinks);
+    Sight see = sight_of(pos, len, p.causal, p.window, p.sinks);
+    if (p.common) see.lo = p.common;
     const int a_steps = (see.first + S::STEP - 1) / S::STEP, b_first = max(see.lo / S::STEP, a_steps);
     const int steps = a_steps + max(0, (see.hi + S::STEP - 1) / S::STEP - b_first);
-    const int chunk = max(p.chunk, (steps + p.parts - 1) / p.parts);
-    if (steps <= chunk) return;
-    const int parts = (steps + chunk - 1) / chunk;
+    const int most = p.parts - p.common_parts, chunk = max(p.chunk, (steps + most - 1) / most);
+    if (steps <= chunk && !p.common) return;
+    const int parts = p.common_parts + (steps + chunk - 1) / chunk;
     const float* ml = p.part_ml + 2 * cell * p.parts;
     float m = kNone;
     for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[2 * i]);
@@ -435,7 +447,7 @@ int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }
 int launch_attention(const AttnParams& p, hipStream_t s) {
     if (p.tiled) return p.f16 ? launch_tiles_f16(p, s) : launch_tiles_f32(p, s);
     const int64_t across = p.by_token ? p.heads : p.kv_heads;
-    const int64_t blocks = (across * p.parts + 7) / 8 * 8 * (int64_t)p.tiles * p.batch;
+    const int64_t blocks = (across * (p.parts - p.common_parts) + 7) / 8 * 8 * (int64_t)p.tiles * p.batch + (across * p.common_parts + 7) / 8 * 8 * (int64_t)p.common_tiles;
     if (blocks <= 0) return 0;
     if (blocks > 0x7fffffff) return -2;
 #define FYN_ATTN(T, D) launch_steps<T, D>(p, (unsigned)blocks, s)

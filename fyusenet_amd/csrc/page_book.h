@@ -40,6 +40,7 @@ class PageBook {
     int batch_rows() const { return words[first_at() + batch_size()]; }
     int pages_free() const { return (int)free_.size(); }
     int pages_used() const { return pages_ - (int)free_.size(); }
+    int common_pages() const { return common_; }                  // that all sequences of the batch begin with
     bool shares() const { return entries_ > pages_used(); }   // some page is in two lists
     int pages_of(int tokens) const { return (int)(((int64_t)tokens + page_tokens_ - 1) / page_tokens_); }
     const std::vector<int>& list(int s) const { return lists_[s]; }
@@ -95,6 +96,12 @@ class PageBook {
         }
         put(first_at() + n, row);
         put(first_at() + sequences_ + 1, n);
+        common_ = n > 1 ? (int)lists_[seqs[0]].size() : 0;
+        for (int i = 1; i < n && common_ > 0; i++) {
+            const std::vector<int>&a = lists_[seqs[0]], &b = lists_[seqs[i]];
+            const int most = std::min(common_, (int)b.size());
+            common_ = (int)(std::mismatch(a.begin(), a.begin() + most, b.begin()).first - a.begin());
+        }
         return moves;
     }
 
@@ -220,6 +227,7 @@ class PageBook {
   private:
     int pages_, sequences_, page_tokens_, most_tokens_, pitch_;
     int64_t entries_ = 0;       // of all lists
+    int common_ = 0;
     std::vector<std::vector<int>> lists_;
     std::vector<int> shared_;   // sequences that have a page
     std::vector<int> free_;     // (a stack: the page that was freed last is taken first)

@@ -52,6 +52,9 @@ struct AttnParams {
     int once;               // no key is read by two workgroups
     int chunk;              // key steps of one part
     int parts;              // most parts of a row
+    // Sequences that begin with the same `common` tokens (a multiple of 32, in the same pages), one new token each: columns are heads
+    // of all of them over those tokens, divided into the first `common_parts` of each row's parts.
+    int common, common_parts, common_chunk, common_tiles;
     float* part_o;          // [row * heads + head][part][dim]
     float* part_ml;         // ... [2]: maximum and sum
 };

@@ -214,11 +214,42 @@ static void branches() {
     CHECK(n.book.batch_size() == 0 && n.book.batch_rows() == 0);
 }
 
+// Pages that all sequences of a batch begin with, at random.
+static void common(unsigned seed) {
+    std::mt19937 gen(seed);
+    auto upto = [&](int n) { return (int)(gen() % (unsigned)(n + 1)); };
+    Model m(400, 6, 8, 400);
+    m.extend({0}, {40 + upto(60)});
+    CHECK(m.book.common_pages() == 0);   // (one sequence)
+    for (int s = 1; s < 5; s++) m.fork(upto(s - 1), {s}, upto(3) ? -1 : 20);
+    m.extend({5}, {30});
+    for (int round = 0; round < 20; round++) {
+        std::vector<int> seqs = {0, 1, 2, 3, 4, 5}, counts;
+        std::shuffle(seqs.begin(), seqs.end(), gen);
+        seqs.resize(upto(6));
+        for (size_t i = 0; i < seqs.size(); i++) counts.push_back(upto(2) ? 1 : upto(9));
+        m.extend(seqs, counts);
+        int want = 0;
+        while (seqs.size() > 1) {
+            bool all = true;
+            for (int s : seqs) all = all && want < (int)m.book.list(s).size() && m.book.list(s)[want] == m.book.list(seqs[0])[want];
+            if (!all) break;
+            want++;
+        }
+        CHECK(m.book.common_pages() == want);
+        m.moved(m.book.compact());
+        m.flush();
+        m.check();
+        CHECK(m.book.common_pages() == want);
+    }
+}
+
 int main(int argc, char** argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "random") for (unsigned s = 0; s < 200; s++) random_run(s);
     else if (what == "refusals") refusals();
     else if (what == "branches") branches();
+    else if (what == "common") for (unsigned s = 0; s < 50; s++) common(s);
     else return 2;
     return 0;
 }

@@ -350,6 +350,51 @@ def test_pages_and_attention_together(typ):
     p.check()
 
 
+#            heads kv dim page prompt branches
+BRANCHES = [
+    (8, 2, 64, 16, 1500, 5),
+    (6, 1, 48, 8, 1024, 7),
+    (4, 4, 128, 64, 2100, 20),
+    (16, 2, 256, 32, 1300, 3),
+    (24, 2, 96, 16, 1055, 4),
+    (20, 1, 40, 8, 1200, 3),      # (more heads of a group than sixteen)
+    (2, 1, 128, 16, 1023, 33),    # (pages in common, and fewer tokens than are worth it)
+    (8, 4, 32, 128, 9000, 17),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("case", BRANCHES, ids=lambda c: "h%d_%d_d%d_p%d_n%d_b%d" % c)
+def test_steps_of_branches(case, typ):
+    """New tokens of sequences that begin with the same pages: of all, of some, in other orders, with one that is not a branch,
+    with one that has grown a long way and one that is cut to what all have."""
+    heads, kv, dim, page, prompt, branches = case
+    others = list(range(1, branches))
+    p = Pair(typ, heads, kv, dim, page, (prompt + 700) // page + 6 * branches + 8, branches + 1)
+    p.cache.extend([0], [prompt], stream=stream())
+    k, v = values(31, typ, (prompt, kv, dim), (prompt, kv, dim))
+    p.cache.write(0, k, v, stream=stream())
+    p.cache.fork(0, others[:-1], stream=stream())
+    p.cache.fork(0, others[-1:], prompt // page * page, stream=stream())
+    for s in range(branches):
+        p.k[s][0], p.v[s][0] = (k, v) if s != others[-1] else (k[:prompt // page * page], v[:prompt // page * page])
+    everyone = list(range(branches))
+    p.extend(everyone, [1] * branches)
+    p.extend([1], [600])
+    p.extend(everyone[::-1], [1] * branches)
+    p.extend([others[-1], 1], [1, 1])
+    p.cache.truncate([others[-1]], [prompt // page * page - 3], stream=stream())
+    p.k[others[-1]][0], p.v[others[-1]][0] = (x[0][:prompt // page * page - 3] for x in (p.k[others[-1]], p.v[others[-1]]))
+    p.extend(everyone, [1] * branches)
+    p.extend([branches], [3])
+    p.extend(everyone, [1] * branches, window=100, sinks=20)
+    p.extend(everyone + [branches], [1] * (branches + 1))
+    p.cache.compact(stream=stream())
+    p.extend(everyone[1:] + [0], [1] * branches, scale=0.2)
+    p.check()
+
+
 @pytest.mark.gpu
 def test_many_sequences_and_pages():
     """More words, rows and moves than one launch's argument holds."""

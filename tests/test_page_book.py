@@ -20,3 +20,8 @@ def program(tmp_path_factory):
 def test_page_book(program, check):
     r = subprocess.run([program, check], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stderr
+
+
+def test_pages_in_common(program):
+    r = subprocess.run([program, "common"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
