@@ -24,9 +24,9 @@ namespace fynhip {
 //
 // Memory bound where a group's heads are the columns: every key and value is read once, in rows of 16 bytes a lane.  The next
 // step's loads are under way while a step is worked on (in the registers that its products have freed).  64 sequences of 32768
-// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 61 us
-// (4.3 TB/s: a workgroup's start, its joins and the unequal lengths weigh there); 16 with a window of 4096, 8 heads of 96, fp32:
-// 74 us (4.8 TB/s).  Sixteen tokens as columns serve short prompts: 12 heads of 197 tokens take 6.7 us, 9.0 in tiles.
+// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 58 us
+// (4.5 TB/s: a workgroup's start, its joins and the unequal lengths weigh there); 16 with a window of 4096, 8 heads of 96, fp32:
+// 74 us (4.8 TB/s).  Over pages that all sequences of a batch begin with, the columns are heads of several sequences.  Sixteen tokens as columns serve short prompts: 12 heads of 197 tokens take 6.7 us, 9.0 in tiles.
 // ---------------------------------------------------------------------------------------------------------------------
 template <class T, int DIMS>
 struct Shape {
@@ -384,23 +384,34 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     }
 }
 
-// The parts of a row of a paged batch: one wave for a row and head, which adds them in their order.  5 us for 24 rows of 32 heads
-// in up to 10 parts: bound by the launch and three loads that wait for each other.
+// The parts of a row of a paged batch: a workgroup for a row and head.  LANES threads have a part's dims, four each, and 256 / LANES
+// parts are added up side by side, those of each in their order, which makes the sums the same ones in every run.  Few bytes in
+// a chain of loads that wait for each other (the batch, the length, the parts): what can be asked for early is.
+// (47 parts for each of 64 rows of 128 dims: the call takes 17 us with both launches; 43 with a wave for a row that takes part after part.)
 template <class T, int DIMS>
 __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
     typedef Shape<T, DIMS> S;
-    const int lane = threadIdx.x & 63;
-    const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int head = (int)(cell % p.heads), n = p.words.first[p.words.sequences + 1];
-    const int64_t row = cell / p.heads;
-    if (row >= p.tokens || n <= 0 || row >= p.words.first[n]) return;
-    int lo = 0, hi = n;   // the sequence whose rows this one is among
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.words.first[mid] <= row) lo = mid;
-        else hi = mid;
+    constexpr int LANES = DIMS == 32 ? 8 : DIMS == 64 ? 16 : DIMS <= 128 ? 32 : 64, SIDE = 256 / LANES;
+    __shared__ f4 sums[256];
+    const int lane = threadIdx.x & 63, cell = blockIdx.x, head = cell % p.heads, row = cell / p.heads;
+    // the sequence whose rows this one is among: the one of that number where each has one new token
+    const int* first = p.words.first;
+    const int n = first[p.words.sequences + 1], guess = min(row, p.words.sequences - 1);
+    const int guess_first = first[guess], guess_end = first[guess + 1], guess_seq = p.words.batch[guess];
+    int end = guess_end, seq = guess_seq;
+    if (n <= 0) return;
+    if (guess >= n || row < guess_first || row >= guess_end) {
+        if (row >= first[n]) return;
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        end = first[lo + 1];
+        seq = p.words.batch[lo];
     }
-    const int len = p.words.len[p.words.batch[lo]], pos = len - (p.words.first[lo + 1] - (int)row);
+    const int len = p.words.len[seq], pos = len - (end - row);
     // the parts that attend_steps made
     Sight see = sight_of(pos, len, p.causal, p.window, p.sinks);
     if (p.common) see.lo = p.common;
@@ -409,25 +420,42 @@ __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
     const int most = p.parts - p.common_parts, chunk = max(p.chunk, (steps + most - 1) / most);
     if (steps <= chunk && !p.common) return;
     const int parts = p.common_parts + (steps + chunk - 1) / chunk;
-    const float* ml = p.part_ml + 2 * cell * p.parts;
+    const float* ml = p.part_ml + 2 * (int64_t)cell * p.parts;
+    const int d = (int)threadIdx.x % LANES * 4, side = (int)threadIdx.x / LANES;
+    const float* from = p.part_o + (int64_t)cell * p.parts * p.dim + d;
+    const bool has = d < p.dim;
+    auto part = [&](int i) { return has && i < parts ? *reinterpret_cast<const f4*>(from + (int64_t)i * p.dim) : f4{0, 0, 0, 0}; };
+    constexpr int AHEAD = 4;
+    f4 ahead[AHEAD];
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++) ahead[t] = part(side + t * SIDE);
+    // (every wave has the maximum and the sum for itself)
     float m = kNone;
     for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[2 * i]);
     for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
     const float base = m == kNone ? 0.f : m;
     float total = 0;
+    for (int i = lane; i < parts; i += 64) total += __builtin_amdgcn_exp2f(ml[2 * i] - base) * ml[2 * i + 1];
+    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
     f4 o = {0, 0, 0, 0};
-    const int d = lane * 4;
-    for (int i = 0; i < parts; i++) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * i] - base);
-        total += f * ml[2 * i + 1];
-        if (d < p.dim) o += *reinterpret_cast<const f4*>(p.part_o + (cell * p.parts + i) * p.dim + d) * f;
+    for (int i = side; i < parts; i += AHEAD * SIDE) {
+#pragma unroll
+        for (int t = 0; t < AHEAD; t++) {
+            if (i + t * SIDE < parts) o += ahead[t] * __builtin_amdgcn_exp2f(ml[2 * (i + t * SIDE)] - base);
+            ahead[t] = part(i + (AHEAD + t) * SIDE);
+        }
     }
-    if (d >= p.dim) return;
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (side > 0 || !has) return;
+    f4 all = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < SIDE; t++) all += sums[t * LANES + threadIdx.x];
     const float inv = total == 0.f ? 0.f : 1.f / total;
     typename Vec<T, 4>::type t;
 #pragma unroll
-    for (int e = 0; e < 4; e++) t[e] = (T)(o[e] * inv);
-    *reinterpret_cast<typename Vec<T, 4>::type*>(reinterpret_cast<T*>(p.out.p) + row * p.out.tok + (int64_t)head * p.out.head + d) = t;
+    for (int e = 0; e < 4; e++) t[e] = (T)(all[e] * inv);
+    *reinterpret_cast<typename Vec<T, 4>::type*>(reinterpret_cast<T*>(p.out.p) + (int64_t)row * p.out.tok + (int64_t)head * p.out.head + d) = t;
 }
 
 template <class T, int DIMS>
@@ -439,7 +467,7 @@ static void launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
     } else {
         hipLaunchKernelGGL((attend_steps<T, DIMS, false, true, false>), dim3(blocks), dim3(256), 0, s, p);
     }
-    if (p.parts > 1) hipLaunchKernelGGL((join_parts<T, DIMS>), dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, s, p);
+    if (p.parts > 1) hipLaunchKernelGGL((join_parts<T, DIMS>), dim3((unsigned)(p.tokens * p.heads)), dim3(256), 0, s, p);
 }
 
 int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }

@@ -468,9 +468,10 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
         p.chunk = (int)std::max(chunk, (longest + parts - 1) / parts);
         p.parts = (int)parts;
         // Branches of one sequence: over the pages that all of them have in front, sixteen columns are heads of several branches, which
-        // reads those pages once for each sixteen instead of once for each branch (32 branches of 12000 tokens, 32 heads of 128
-        // dims in groups of 4: a step of 43 us, and 114 us without).  Rows are joined then that one part would have done, so only
-        // where that many tokens are the same.  A captured call is replayed when the sequences may have no pages in common.
+        // reads those pages once for each sixteen instead of once for each branch (fp16, 32 heads of 128 dims in groups of 4, 12000
+        // tokens in common: 39 us with 32 branches, and 114 without; 17.5 and 17.4 with two).  There is always a second launch
+        // then, so that it takes 1024 such tokens, which have several parts anyway (260: 11.2 and 8.5 us with four branches;
+        // 1040: 11.3 and 11.1, and with 32 of them 14 and 20).  A captured call is replayed when the sequences may have no pages in common.
         int shortest = book_.length(book_.words[book_.batch_at()]);
         for (int b = 0; b < p.batch; b++) shortest = std::min(shortest, book_.length(book_.words[book_.batch_at() + b]));
         const int common = std::min((int64_t)book_.common_pages() * d.page_tokens, (int64_t)shortest - 1) / 32 * 32, together = (p.batch * group + 15) / 16;
