@@ -24,8 +24,8 @@ namespace fynhip {
 //
 // Memory bound where a group's heads are the columns: every key and value is read once, in rows of 16 bytes a lane.  The next
 // step's loads are under way while a step is worked on (in the registers that its products have freed).  64 sequences of 32768
-// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 58 us
-// (4.5 TB/s: a workgroup's start, its joins and the unequal lengths weigh there); 16 with a window of 4096, 8 heads of 96, fp32:
+// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 57 to 64 us
+// (4.1 to 4.6 TB/s: a workgroup's start, its joins and the unequal lengths weigh there); 16 with a window of 4096, 8 heads of 96, fp32:
 // 74 us (4.8 TB/s).  Over pages that all sequences of a batch begin with, the columns are heads of several sequences.  Sixteen tokens as columns serve short prompts: 12 heads of 197 tokens take 6.7 us, 9.0 in tiles.
 // ---------------------------------------------------------------------------------------------------------------------
 template <class T, int DIMS>

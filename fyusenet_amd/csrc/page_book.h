@@ -69,6 +69,9 @@ class PageBook {
         }
         if (rows > 0x7fffffff) refuse(false, "too many tokens in one batch");
         if (need > (int64_t)free_.size()) refuse(true, std::to_string(need) + " pages are wanted, " + std::to_string(free_.size()) + " are free");
+        // (the batch as before: of the pages in common only the last one, which need not be full, may have become a copy)
+        const bool same = n > 1 && batch_size() == n && std::equal(seqs, seqs + n, words.begin() + batch_at());
+        const int known = same ? std::max(0, common_ - 1) : 0;
         Moves moves;
         for (int i = 0; i < n; i++) {
             const int s = seqs[i], len = words[s];
@@ -100,7 +103,7 @@ class PageBook {
         for (int i = 1; i < n && common_ > 0; i++) {
             const std::vector<int>&a = lists_[seqs[0]], &b = lists_[seqs[i]];
             const int most = std::min(common_, (int)b.size());
-            common_ = (int)(std::mismatch(a.begin(), a.begin() + most, b.begin()).first - a.begin());
+            common_ = (int)(std::mismatch(a.begin() + known, a.begin() + most, b.begin() + known).first - a.begin());
         }
         return moves;
     }

@@ -218,7 +218,7 @@ static void branches() {
 static void common(unsigned seed) {
     std::mt19937 gen(seed);
     auto upto = [&](int n) { return (int)(gen() % (unsigned)(n + 1)); };
-    Model m(400, 6, 8, 400);
+    Model m(900, 6, 8, 1000);
     m.extend({0}, {40 + upto(60)});
     CHECK(m.book.common_pages() == 0);   // (one sequence)
     for (int s = 1; s < 5; s++) m.fork(upto(s - 1), {s}, upto(3) ? -1 : 20);
@@ -227,16 +227,29 @@ static void common(unsigned seed) {
         std::vector<int> seqs = {0, 1, 2, 3, 4, 5}, counts;
         std::shuffle(seqs.begin(), seqs.end(), gen);
         seqs.resize(upto(6));
-        for (size_t i = 0; i < seqs.size(); i++) counts.push_back(upto(2) ? 1 : upto(9));
-        m.extend(seqs, counts);
         int want = 0;
-        while (seqs.size() > 1) {
-            bool all = true;
-            for (int s : seqs) all = all && want < (int)m.book.list(s).size() && m.book.list(s)[want] == m.book.list(seqs[0])[want];
-            if (!all) break;
-            want++;
+        for (int again = upto(3); again >= 0; again--) {   // (the same batch some times)
+            counts.clear();
+            for (size_t i = 0; i < seqs.size(); i++) counts.push_back(upto(2) ? upto(1) : upto(9));
+            m.extend(seqs, counts);
+            want = 0;
+            while (seqs.size() > 1) {
+                bool all = true;
+                for (int s : seqs) all = all && want < (int)m.book.list(s).size() && m.book.list(s)[want] == m.book.list(seqs[0])[want];
+                if (!all) break;
+                want++;
+            }
+            CHECK(m.book.common_pages() == want);
+            if (upto(9) == 0 && !seqs.empty()) {   // one of them is cut, or ends and becomes a branch of another
+                const int s = seqs[upto((int)seqs.size() - 1)], other = (s + 1 + upto(4)) % 6, keep = upto(1) ? 0 : m.book.length(s) / 2;
+                m.book.truncate(1, &s, &keep);
+                m.flush();
+                m.want[s].resize(keep);
+                if (!keep && m.book.length(other)) m.fork(other, {s}, upto(1) ? -1 : m.book.length(other) / 2);
+                m.check();
+                want = m.book.common_pages();
+            }
         }
-        CHECK(m.book.common_pages() == want);
         m.moved(m.book.compact());
         m.flush();
         m.check();
