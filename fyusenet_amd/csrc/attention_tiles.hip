@@ -13,11 +13,11 @@
 // read one piece of sixteen rows (keys), or pieces side by side of eight rows (values), find them in different banks.  Values in
 // 16 bits are turned by the LDS as they are read: four keys of a dim to a lane, which had four dims of a key.
 //
-// Bound by the matrix unit and, beside it, the exponentials (a unit of 32 keys by 32 queries, 128 dims: 512 cycles of matrix
-// instructions, about 400 of vector ones), with two waves on each SIMD to overlap them: 16384 tokens, 16 heads of 128, causal, fp16
-// 1.22 ms, 905 TFLOP/s (a large library product of 16-bit matrices: 1173).  Of larger tiles and other orders, with 4096 tokens,
-// 16 heads of 128: 32 keys a wave 159 us, 64 keys 166; through registers and turned there 172; the next unit's first product in
-// front of this one's exponentials 192 (its registers spill).  fp32, whose matrix instructions are a sixteenth as fast: 4096 tokens, 8
+// In 16 bits a weight goes into the second product as two numbers (22 bits of it; one alone, 11 bits, is 2.6e-4 off the formula in 64
+// bits where two are 1.9e-4, which is the result's own rounding), so that a unit of 32 keys by 32 queries, 128 dims, has 24 matrix
+// instructions, 768 cycles.  16384 tokens, 16 heads of 128, causal, fp16: 1.69 ms (1.24 with one number).  Of larger tiles and other
+// orders, with one number, 4096 tokens, 16 heads of 128: 32 keys a wave 159 us, 64 keys 166; through registers and turned there 172; the
+// next unit's first product in front of this one's exponentials 192 (its registers spill).  fp32, whose matrix instructions are a sixteenth as fast: 4096 tokens, 8
 // heads of 128, 685 us, 100 TFLOP/s (library: 154).
 #include "attention_common.h"
 
@@ -273,35 +273,36 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
                     for (int r = 0; r < 16; r++) acc[d][r] *= alpha;
             }
-            // Weights 2^6 times as large as relative to m: 16 bits hold them to full precision down to 2^-20 of it.
-            // They are rounded to 16 bits for the second product, and it is the rounded ones that are summed up.
+            // Weights 2^6 times as large as relative to m.  In 16 bits a weight is two numbers, what the first one's rounding takes from it
+            // is the second: 22 bits of it in all down to 2^-9 of the largest weight, and never off by more than 2^-31 of that one.
             const float base = m == kNone ? 0.f : m - 6.f;
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -base));
+            float sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < 16; r++) sum[r & 3] += sc[r];
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if constexpr (F16) {
-                h8 w[2];
+                h8 w[2], rest[2];
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const h2 two = {(_Float16)sc[t * 8 + e], (_Float16)sc[t * 8 + e + 1]};
-                        l = __builtin_amdgcn_fdot2(two, h2{(_Float16)1, (_Float16)1}, l, false);
-                        w[t][e] = two[0];
-                        w[t][e + 1] = two[1];
+                    for (int e = 0; e < 8; e++) {
+                        w[t][e] = (_Float16)sc[t * 8 + e];
+                        rest[t][e] = (_Float16)(sc[t * 8 + e] - (float)w[t][e]);
                     }
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int d = 0; d < S::DIM_TILES; d++) {
                         acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], w[t], acc[d], 0, 0, 0);
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], rest[t], acc[d], 0, 0, 0);
                         if (t == 0) {
                             vf[d] = value(1, d);
                             if (AHEAD) __builtin_amdgcn_sched_barrier(0);
                         }
                     }
             } else {
-#pragma unroll
-                for (int r = 0; r < 16; r++) l += sc[r];
 #pragma unroll
                 for (int r = 0; r < 16; r++)
 #pragma unroll

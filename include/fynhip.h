@@ -314,7 +314,8 @@ int fyn_layer_kernel_info(fyn_net* net, int layer, char* buf, size_t buflen);
  *
  * The calls take device memory and enqueue on a stream of the caller's (a hipStream_t, NULL: the default stream of the
  * device); they return before the work is done.  The device is the one that the memory (or the cache) is on, whichever is
- * current.  Sums and weights are held in 32 bits whatever the storage.
+ * current.  Scores, maxima, weights and sums are computed and held in 32 bits whatever the storage; with 16-bit storage a weight is
+ * multiplied with the values as two 16-bit numbers, which are 22 bits of it (and off by 2^-31 of the row's largest weight at most).
  *
  * A token at position i of n sees position j where j < n, and, if causal, j <= i, and, with a window > 0, |i - j| < window
  * or j < sinks (the first tokens, which stay visible).  A query that sees nothing gives zero.  What a token does not see
