@@ -174,7 +174,9 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     const int64_t v_pitch = PAGED ? row_bytes : p.v.tok * (int64_t)sizeof(T);
     KVec k[S::TILES][S::KLOADS];
     VVec v[S::TILES][4][S::BLOCKS];
-    // (pieces behind a head's last value are taken from within it: they meet queries that are zero, or end in dims that nobody stores)
+    // Pieces behind a head's last value are taken from within it.  Of the values they end in dims that nobody stores; of the keys they are
+    // zero in the product, as the queries are (zero times an infinity of the head's own would not be).
+    auto has_piece = [&](int s) { return (s + 1) * 4 * S::VEC <= S::LEAST || (s * 4 + g) * S::VEC < p.dim; };
     auto load_keys = [&](const Where& w) {
 #pragma unroll
         for (int t = 0; t < S::TILES; t++)
@@ -212,11 +214,12 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
             sc[t] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < S::KLOADS; s++) {
+                const KVec piece = has_piece(s) ? k[t][s] : KVec{};
                 if constexpr (F16) {
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece, q[s], sc[t], 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][s][e], q[s][e], sc[t], 0, 0, 0);
+                    for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[e], q[s][e], sc[t], 0, 0, 0);
                 }
             }
             sc[t] *= p.scale_log2;

@@ -41,6 +41,7 @@ struct TileShape {
     static_assert(ALL % 256 == 0 || ALL < 256, "whole waves load");
     static constexpr int HALF = 2 * TILE * PITCH * 16;                           // bytes of a tile: keys, then values
     static constexpr int DIM_TILES = DIMS / 32;
+    static constexpr int LEAST = DIMS == 256 ? 128 : DIMS - 32;                  // fewer dims than any head of the class has
     static_assert(KW == 1 || HALF >= 2 * DIM_TILES * 4096, "sums of two waves in the place of a tile");
     static constexpr int LDS = 2 * HALF;
     static_assert(LDS + 2048 <= 160 * 1024, "a CU's LDS");
@@ -137,8 +138,8 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
     auto at_of = [&](int st) { return (st < a_steps ? st : b_first + st - a_steps) * S::TILE; };
 
     // A tile on its way: a lane's sixteen bytes go to the place that its number says, so the exchange of pieces is one of what it
-    // asks for.  (Pieces behind a head's last value are taken from within it: in the first product they meet queries that are zero
-    // there, in the second they end in dims that nobody stores.)
+    // asks for.  (Pieces behind a head's last value are taken from within it: of the keys they are zero in the first product, as
+    // the queries are, because zero times an infinity of the head's own would not be; of the values they end in dims that nobody stores.)
     const int row_bytes = p.dim * (int)sizeof(T);
     constexpr int ROWS = 64 / S::PITCH;   // of a load
     const int lane_row = lane / S::PITCH, lane_piece = lane % S::PITCH;
@@ -226,11 +227,12 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
             if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < S::PIECES / 2; s++) {
+                const KVec piece = (2 * s + 2) * S::VEC <= S::LEAST || (2 * s + half) * S::VEC < p.dim ? kf[s] : KVec{};
                 if constexpr (F16) {
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s], q[s], sc, 0, 0, 0);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(piece, q[s], sc, 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[s][e], q[s][e], sc, 0, 0, 0);
+                    for (int e = 0; e < 4; e++) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[e], q[s][e], sc, 0, 0, 0);
                 }
             }
             if (!((at >= all.lo && at + 32 <= all.hi) || at + 32 <= all.first)) {
