@@ -259,15 +259,17 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
         const float m_new = fmaxf(m, top), base = m_new == kNone ? 0.f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m - base);   // (m = none: 0)
         m = m_new;
-        // Weights are kept 2^14 times as large: in 16 bits they then have their full precision down to 2^-28 of the
-        // largest, and what rounding takes from them is a second operand of the product.
+        // In 16 bits weights are kept 2^14 times as large: they then have their full precision down to 2^-28 of the largest, and
+        // what rounding takes from them is a second operand of the product.  (In 32 bits nothing is gained by that, and the
+        // exponent's argument would lose three bits: 14 has steps of 2^-20.)
+        constexpr float shift = F16 ? 14.f : 0.f;
         f4 w[S::TILES];
         float sum = 0;
 #pragma unroll
         for (int t = 0; t < S::TILES; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                w[t][r] = __builtin_amdgcn_exp2f(sc[t][r] - base + 14.f);
+                w[t][r] = __builtin_amdgcn_exp2f(sc[t][r] - base + shift);
                 sum += w[t][r];
             }
         l = l * alpha + sum;

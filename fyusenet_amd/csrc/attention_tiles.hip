@@ -24,7 +24,6 @@
 namespace fynhip {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr float kLag = 8.f;   // binary orders of magnitude
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
@@ -45,6 +44,9 @@ struct TileShape {
     static_assert(KW == 1 || HALF >= 2 * DIM_TILES * 4096, "sums of two waves in the place of a tile");
     static constexpr int LDS = 2 * HALF;
     static_assert(LDS + 2048 <= 160 * 1024, "a CU's LDS");
+    // Weights are 2^SHIFT times as large as relative to the running maximum, which may be LAG binary orders of magnitude behind the true
+    // one.  (In 32 bits both are 0: the larger the exponent's argument is, the fewer bits it has behind the point.)
+    static constexpr float SHIFT = F16 ? 6.f : 0.f, LAG = F16 ? 8.f : 0.f;
     static constexpr int WAVES = DIMS <= (F16 ? 128 : 64) && LDS <= 64 * 1024 ? 2 : 1;   // workgroups that share a CU (their registers)
 };
 
@@ -264,10 +266,10 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, sc[r]);
             top = across(top) * scale;
-            // The sums are relative to a maximum that may be the true one's 2^-8 (with weights up to 2^14 then): it follows where a
-            // query is further off, which after the first tiles is seldom.
-            if (__any(top > m + kLag)) {
-                const float m_new = top > m + kLag ? top : m, alpha = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - m_new);   // (by each query alone)
+            // In 16 bits the sums are relative to a maximum that may be the true one's 2^-8 (with weights up to 2^14 then): it follows where
+            // a query is further off, which after the first tiles is seldom.
+            if (__any(top > m + S::LAG)) {
+                const float m_new = top > m + S::LAG ? top : m, alpha = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - m_new);   // (by each query alone)
                 m = m_new;
                 l *= alpha;
 #pragma unroll
@@ -275,9 +277,9 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
                     for (int r = 0; r < 16; r++) acc[d][r] *= alpha;
             }
-            // Weights 2^6 times as large as relative to m.  In 16 bits a weight is two numbers, what the first one's rounding takes from it
-            // is the second: 22 bits of it in all down to 2^-9 of the largest weight, and never off by more than 2^-31 of that one.
-            const float base = m == kNone ? 0.f : m - 6.f;
+            // In 16 bits a weight is 2^6 times as large as relative to m, and two numbers: what the first one's rounding takes from it
+            // is the second, 22 bits of it in all down to 2^-9 of the largest weight, and never off by more than 2^-31 of that one.
+            const float base = m == kNone ? 0.f : m - S::SHIFT;
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -base));
             float sum[4] = {0, 0, 0, 0};

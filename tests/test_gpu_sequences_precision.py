@@ -129,3 +129,50 @@ def test_pieces_over_the_cache_keep_their_weights(case, typ):
         ks, vs = torch.cat([k0[a:a + old], k1[b:b + new]]), torch.cat([v0[a:a + old], v1[b:b + new]])
         close(out[b:b + new], *exact(q1[b:b + new], ks, vs, old, (old + new) // 2 + 100, True, window, sinks), "sequence at %d" % b)
         a, b = a + old, b + new
+
+
+# Two weights that differ by a few of the steps that a number of 32 bits near one has, with values 1 and -1: a result that is their difference.
+# Of the largest weight's neighbours exp gives 1 - x to a step, 2^-24 there (and may be one step off), so the difference is off by 2 steps at
+# most, half of that in the result of two keys; the rest is rounded in proportion.
+#   heads tokens batch: sixteen columns, 64 and 128 queries a workgroup
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,tokens,heads", [(1, 40, 2), (4, 130, 32), (6, 160, 48)])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("later", [0.0, 7.0])
+def test_weights_of_32_bits_keep_their_bits(batch, tokens, heads, dim, later):
+    """32-bit storage.  later: how much smaller, in powers of two, the weights are that a sequence begins with."""
+    first = 33 if later else 0      # (more than one step of keys)
+    for steps in (3.3, 5.7, 20.4):
+        x = steps * 2.0 ** -24
+        q, k, v = (torch.zeros(batch, tokens, n, dim, device="cuda") for n in (heads, 1, 1))
+        q[..., 0] = 1
+        k[:, :first, 0, 0] = -later * math.log(2)
+        k[:, first + 2:, 0, 0] = -80.0
+        k[:, first + 1, 0, 0] = -x                          # (exactly: the product with one)
+        v[:, first], v[:, first + 1] = 1, -1
+        out = torch.empty_like(q)
+        fa.attention(q, k, v, out, causal=False, scale=1.0, stream=stream())
+        want = -math.expm1(-x) / (1 + math.exp(-x) + first * 2.0 ** -later)
+        off = (out.double() - want).abs().max()
+        assert float(off) <= 2 * 2.0 ** -24 / (2 + first * 2.0 ** -later) + 2.0 ** -22 * want, "%g steps: off by %.3g of %.3g" % (steps, off, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 64, 136])
+def test_weights_of_32_bits_over_the_cache(dim):
+    for steps in (3.3, 5.7, 20.4):
+        x, n = steps * 2.0 ** -24, 150
+        c = fa.SequenceCache(STORAGE["f32"], 1, 4, 2, dim, 16, 10, 1)
+        k, v, q = (torch.zeros(m, h, dim, device="cuda") for m, h in ((n, 2), (n, 2), (1, 4)))
+        q[..., 0] = 1
+        k[..., 0], k[77, :, 0], k[78, :, 0] = -80.0, 0.0, -x
+        v[77], v[78] = 1, -1
+        c.extend([0], [n - 1], stream=stream())
+        c.write(0, k[:-1], v[:-1], stream=stream())
+        c.extend([0], [1], stream=stream())
+        c.write(0, k[-1:], v[-1:], stream=stream())
+        out = torch.empty_like(q)
+        c.attend(0, q, out, scale=1.0, stream=stream())
+        want = -math.expm1(-x) / (1 + math.exp(-x))
+        off = (out.double() - want).abs().max()
+        assert float(off) <= 2.0 ** -24 + 2.0 ** -22 * want, "%g steps: off by %.3g of %.3g" % (steps, off, want)
