@@ -374,6 +374,14 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
         f4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; w++) o += *reinterpret_cast<const f4*>(&sums[w][col][d]) * f[w];
+        if (!zero && total == total && (o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
+            Sight see = together ? any : sight_of(pos0 + o_tok, len, p.causal, p.window, p.sinks);
+            if (BRANCHES && p.common && !together) see.lo = p.common;
+            const int second = b_first - a_steps;   // (steps of the window are so many further on)
+            o = with_infinities<T>(o, see, begin * S::STEP, min(min(end, a_steps) * S::STEP, most), (second + max(begin, a_steps)) * S::STEP, min((second + end) * S::STEP, most),
+                                   [&](int j) { return reinterpret_cast<const T*>(PAGED ? vbase + table[j >> p.pages.shift] * p.pages.page_bytes + (j & ((1 << p.pages.shift) - 1)) * row_bytes
+                                                                                        : vbase + j * p.v.tok * (int64_t)sizeof(T)) + d; });
+        }
         if (only) {
             typename Vec<T, 4>::type t;
 #pragma unroll
@@ -446,7 +454,12 @@ __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
     for (int i = side; i < parts; i += AHEAD * SIDE) {
 #pragma unroll
         for (int t = 0; t < AHEAD; t++) {
-            if (i + t * SIDE < parts) o += ahead[t] * __builtin_amdgcn_exp2f(ml[2 * (i + t * SIDE)] - base);
+            if (i + t * SIDE < parts) {
+                const float f = __builtin_amdgcn_exp2f(ml[2 * (i + t * SIDE)] - base);
+                // (a part's infinity stays one, however little the part weighs; a part without weights has none)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] += f == 0.f && __builtin_isinf(ahead[t][e]) ? ahead[t][e] : ahead[t][e] * f;
+            }
             ahead[t] = part(i + (AHEAD + t) * SIDE);
         }
     }

@@ -42,6 +42,38 @@ template <> struct Vec<float, 2> { typedef f2 type; };
 __device__ __forceinline__ bool finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
 __device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000) != 0x7f800000; }
 
+// Four values of a result, of which some are NaN though no score is.  A weight that a key's score gives is above zero, but 32 or 16 bits may
+// hold it as zero, or what rounding took from it is zero or below: then an infinite value makes NaN where the sum is infinite.  Here it is
+// looked up again: what the query sees of the positions [from, to) and [from2, to2) are infinities of one sign, or not (NaN among them).
+// src(j): where the four values of position j are.
+template <class T, class Src>
+__device__ __forceinline__ f4 with_infinities(f4 o, const Sight& see, int from, int to, int from2, int to2, Src src) {
+    unsigned odd = 0, nan = 0, up = 0, down = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) odd |= o[e] != o[e] ? 1u << e : 0u;
+    for (int part = 0; part < 2; part++) {
+        const int a = part ? from2 : from, z = part ? to2 : to;
+        for (int j = a; j < z && (odd & ~(nan | (up & down))); j += 8) {
+            typename Vec<T, 4>::type x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = *reinterpret_cast<const typename Vec<T, 4>::type*>(src(min(j + i, z - 1)));
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const T v = x[i][e];
+                    if (finite(v) || j + i >= z || !see.sees(j + i)) continue;
+                    (v > (T)0 ? up : v < (T)0 ? down : nan) |= 1u << e;
+                }
+        }
+    }
+    const float inf = __builtin_huge_valf();
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if ((odd & ~(nan | (up & down)) & (up | down)) >> e & 1) o[e] = up >> e & 1 ? inf : -inf;
+    return o;
+}
+
 // A sequence of the batch: its tokens, and its queries: `count` rows from row0 of q and the result, the first of them at
 // position pos0.
 struct Batched {

@@ -376,6 +376,7 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
     }
     if (tok >= in.count) return;
     const bool zero = tok >= seen_rows;
+    bool odd = false;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = reinterpret_cast<T*>(p.out.p) + (PAGED ? 0 : b * p.out.seq) + (int64_t)(in.row0 + tok) * p.out.tok + (int64_t)head * p.out.head;
 #pragma unroll
@@ -387,9 +388,24 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
             typename Vec<T, 4>::type t;
 #pragma unroll
             for (int e = 0; e < 4; e++) t[e] = zero ? (T)0 : (T)(acc[d][4 * j + e] * inv);
-            if (dim < p.dim) *reinterpret_cast<typename Vec<T, 4>::type*>(dst + dim) = t;
+            if (dim < p.dim) {
+                *reinterpret_cast<typename Vec<T, 4>::type*>(dst + dim) = t;
+#pragma unroll
+                for (int e = 0; e < 4; e++) odd = odd || t[e] != t[e];
+            }
         }
     }
+    // (seldom: from what has been stored, so that no sum is kept for it)
+    if (odd && l == l)
+        for (int dim = 4 * half; dim < p.dim; dim += 8) {
+            if (dim / 32 % S::KW != mates) continue;
+            auto& at = *reinterpret_cast<typename Vec<T, 4>::type*>(dst + dim);
+            const typename Vec<T, 4>::type t = at;
+            if (t[0] == t[0] && t[1] == t[1] && t[2] == t[2] && t[3] == t[3]) continue;
+            const f4 o = with_infinities<T>(f4{(float)t[0], (float)t[1], (float)t[2], (float)t[3]}, mine, 0, mine.first, mine.lo, mine.hi,
+                                            [&](int j) { return reinterpret_cast<const T*>(row(vbase, p.v.tok, j, 0, 0)) + dim; });
+            at = typename Vec<T, 4>::type{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
+        }
 }
 
 template <class T, int DIMS, int QW>

@@ -319,7 +319,8 @@ int fyn_layer_kernel_info(fyn_net* net, int layer, char* buf, size_t buflen);
  *
  * A token at position i of n sees position j where j < n, and, if causal, j <= i, and, with a window > 0, |i - j| < window
  * or j < sinks (the first tokens, which stay visible).  A query that sees nothing gives zero.  What a token does not see
- * has no influence, whatever the memory holds there (infinities and NaN included).  Query head h uses key head
+ * has no influence, whatever the memory holds there (infinities and NaN included); an infinite value that it sees makes the result
+ * infinite, however little it weighs, and NaN beside one of the other sign.  Query head h uses key head
  * h / (heads / kv_heads). */
 
 /* Rows of a tensor: element (sequence, token, head, x) is at sequence*sequence_pitch + token*token_pitch + head*head_pitch + x,
