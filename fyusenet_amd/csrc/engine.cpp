@@ -1038,6 +1038,7 @@ void Net::time_layer(int layer_no, int iters, float* ms) {
     if (!is_setup) fail(FYN_ERR_STATE, "time_layer() before setup()");
     FYN_HIP(hipSetDevice(device));
     Layer* l = layer(layer_no);
+    l->before_pass(stream);
     // The launches are captured into one hipGraph so that host-side dispatch gaps do not enter the
     // measurement; the events bracket the graph on the network's stream.
     hipGraph_t g = nullptr;

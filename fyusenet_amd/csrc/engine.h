@@ -103,7 +103,7 @@ class Layer {
     virtual const FuncParams* pointwise() const { return nullptr; }
     virtual void computed_by(int) {}
     virtual void bind_cache(std::shared_ptr<Cache>, int) { fail(FYN_ERR_INVALID, "layer %s (%d) is not an attention layer", d.name, d.number); }
-    virtual void before_pass(hipStream_t) {}   // (Net::with_cache) on the host, before the layers run or are replayed
+    virtual void before_pass(hipStream_t) {}   // (Net::with_cache) on the host, before the layers run or are replayed, or one of them is timed
     Act act() const;
     const Tensor& tin(int port) const;
     const Tensor& tout() const;

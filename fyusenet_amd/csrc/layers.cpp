@@ -689,6 +689,7 @@ class AttentionLayer : public Layer {
         if (cache) w.push_back(this);
     }
     void before_pass(hipStream_t s) override {
+        if (!cache) return;
         // (a captured pass is for a batch of as many sequences with as many new tokens each)
         std::vector<int> now = cache->expect(oh * ow, s);
         if (now == first) return;
