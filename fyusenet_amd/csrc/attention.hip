@@ -477,15 +477,11 @@ __global__ __launch_bounds__(256) void join_parts(const AttnParams p) {
 }
 
 template <class T, int DIMS>
-static void launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
-    if (p.paged) {
-        if (p.by_token) hipLaunchKernelGGL((attend_steps<T, DIMS, true, true, false>), dim3(blocks), dim3(256), 0, s, p);
-        else if (p.once) hipLaunchKernelGGL((attend_steps<T, DIMS, true, false, true>), dim3(blocks), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((attend_steps<T, DIMS, true, false, false>), dim3(blocks), dim3(256), 0, s, p);
-    } else {
-        hipLaunchKernelGGL((attend_steps<T, DIMS, false, true, false>), dim3(blocks), dim3(256), 0, s, p);
-    }
-    if (p.parts > 1) hipLaunchKernelGGL((join_parts<T, DIMS>), dim3((unsigned)(p.tokens * p.heads)), dim3(256), 0, s, p);
+static hipError_t launch_steps(const AttnParams& p, unsigned blocks, hipStream_t s) {
+    const auto kernel = !p.paged ? attend_steps<T, DIMS, false, true, false> : p.by_token ? attend_steps<T, DIMS, true, true, false>
+                        : p.once ? attend_steps<T, DIMS, true, false, true> : attend_steps<T, DIMS, true, false, false>;
+    const hipError_t e = start(kernel, blocks, s, p);
+    return e != hipSuccess || p.parts <= 1 ? e : start(join_parts<T, DIMS>, (unsigned)(p.tokens * p.heads), s, p);
 }
 
 int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }
@@ -496,7 +492,8 @@ int launch_attention(const AttnParams& p, hipStream_t s) {
     const int64_t blocks = (across * (p.parts - p.common_parts) + 7) / 8 * 8 * (int64_t)p.tiles * p.batch + (across * p.common_parts + 7) / 8 * 8 * (int64_t)p.common_tiles;
     if (blocks <= 0) return 0;
     if (blocks > 0x7fffffff) return -2;
-#define FYN_ATTN(T, D) launch_steps<T, D>(p, (unsigned)blocks, s)
+    hipError_t e;
+#define FYN_ATTN(T, D) e = launch_steps<T, D>(p, (unsigned)blocks, s)
     if (p.f16) {
         if (p.dim <= 32) FYN_ATTN(_Float16, 32);
         else if (p.dim <= 64) FYN_ATTN(_Float16, 64);
@@ -511,7 +508,7 @@ int launch_attention(const AttnParams& p, hipStream_t s) {
         else FYN_ATTN(float, 256);
     }
 #undef FYN_ATTN
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return e == hipSuccess ? 0 : -1;
 }
 
 }  // namespace fynhip

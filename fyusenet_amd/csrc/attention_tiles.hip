@@ -409,9 +409,8 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 }
 
 template <class T, int DIMS, int QW>
-static void launch_tiles(const AttnParams& p, unsigned blocks, hipStream_t s) {
-    if (p.paged) hipLaunchKernelGGL((attend_tiles<T, DIMS, true, QW>), dim3(blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((attend_tiles<T, DIMS, false, QW>), dim3(blocks), dim3(256), 0, s, p);
+static hipError_t launch_tiles(const AttnParams& p, unsigned blocks, hipStream_t s) {
+    return start(p.paged ? attend_tiles<T, DIMS, true, QW> : attend_tiles<T, DIMS, false, QW>, blocks, s, p);
 }
 
 #if FYN_ATTN_HALF
@@ -427,16 +426,17 @@ static int launch_class(const AttnParams& p, hipStream_t s) {
     const int64_t blocks = ((int64_t)p.batch * p.heads + 7) / 8 * 8 * p.tiles;
     if (blocks <= 0) return 0;
     if (blocks > 0x7fffffff) return -2;
-    if (p.dim <= 32) launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 64) launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 96) launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 128) launch_tiles<Stored, 128, QW>(p, (unsigned)blocks, s);
+    hipError_t e;
+    if (p.dim <= 32) e = launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 64) e = launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 96) e = launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);
+    else if (p.dim <= 128) e = launch_tiles<Stored, 128, QW>(p, (unsigned)blocks, s);
 #if FYN_ATTN_HALF
-    else launch_tiles<Stored, 256, QW>(p, (unsigned)blocks, s);
+    else e = launch_tiles<Stored, 256, QW>(p, (unsigned)blocks, s);
 #else
     else return -1;   // (queries and sums of 32 bits: more registers than a wave has)
 #endif
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return e == hipSuccess ? 0 : -1;
 }
 
 int FYN_ATTN_NAME(const AttnParams& p, hipStream_t s) { return p.tiled == 128 ? launch_class<4>(p, s) : launch_class<2>(p, s); }

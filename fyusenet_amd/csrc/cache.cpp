@@ -143,8 +143,7 @@ Cache::Cache(int dev, const fyn_cache_desc& desc)
         FYN_HIP(hipMalloc(&words_, book_.words.size() * sizeof(int)));
         FYN_HIP(hipMalloc(&parts_, (size_t)(part_cells_ * (d.head_dim + 2)) * sizeof(float)));
         FYN_HIP(hipEventCreateWithFlags(&between_, hipEventDisableTiming));
-        launch_fill_zero(words_, book_.words.size() * sizeof(int), nullptr);
-        FYN_HIP(hipGetLastError());
+        FYN_HIP(hipMemset(words_, 0, book_.words.size() * sizeof(int)));
         FYN_HIP(hipStreamSynchronize(nullptr));
     } catch (...) {
         release();
@@ -170,7 +169,9 @@ Cache::~Cache() {
 
 static bool capturing(hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) == hipSuccess) return st != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();
+    return false;
 }
 
 void Cache::join_streams(hipStream_t s) {
@@ -223,7 +224,7 @@ void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, i
     CacheChange c;
     auto clear = [&] { c.runs = c.singles = c.lists = c.moves = 0; };
     auto send = [&] {
-        if (c.used()) launch_cache_change(m, c, s);
+        if (c.used()) FYN_HIP(launch_cache_change(m, c, s));
         clear();
     };
     clear();
@@ -266,7 +267,6 @@ void Cache::carry_out(const PageBook::Moves& moves, hipStream_t s, int source, i
         c.moves++;
     }
     send();
-    FYN_HIP(hipGetLastError());
 }
 
 PageLayout Cache::layout(int layer) const {
@@ -360,8 +360,7 @@ void Cache::write(int layer, const fyn_rows& k, const fyn_rows& v, int rows, hip
     p.k = rows_of(k); p.v = rows_of(v);
     p.words = words();
     p.rows = rows; p.kv_heads = d.kv_heads; p.dim = d.head_dim; p.f16 = f16;
-    launch_cache_write(p, s);
-    FYN_HIP(hipGetLastError());
+    FYN_HIP(launch_cache_write(p, s));
 }
 
 void Cache::read(int n, const int* seqs, int layer, const fyn_rows& k, const fyn_rows& v, int rows, hipStream_t s) {
@@ -397,10 +396,9 @@ void Cache::read(int n, const int* seqs, int layer, const fyn_rows& k, const fyn
         }
         r.first[r.n] = at;
         p.rows = at;
-        launch_cache_read(p, r, s);
+        FYN_HIP(launch_cache_read(p, r, s));
         row += at;
     }
-    FYN_HIP(hipGetLastError());
 }
 
 // Steps of keys that a token at `pos` of a sequence takes, as the kernel counts them.

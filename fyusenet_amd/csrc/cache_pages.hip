@@ -56,18 +56,16 @@ __global__ __launch_bounds__(256) void change_cache(const CacheMemory m, const C
 }
 
 template <int WORDS>
-static void launch_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
+static hipError_t launch_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
     ChangeArgument<WORDS> a;
     a.runs = c.runs; a.singles = c.singles; a.lists = c.lists; a.moves = c.moves; a.source = c.source; a.entries = c.entries;
     for (int i = 0; i < c.used(); i++) a.w[i] = c.w[i];
     const int64_t parts = (m.page_bytes + kPart - 1) / kPart;
-    hipLaunchKernelGGL(change_cache<WORDS>, dim3((unsigned)(1 + c.lists + c.moves * parts)), dim3(256), 0, s, m, a, (int)parts);
+    return start(change_cache<WORDS>, (unsigned)(1 + c.lists + c.moves * parts), s, m, a, (int)parts);
 }
 
-void launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
-    if (c.used() <= 48) launch_change<48>(m, c, s);
-    else if (c.used() <= 240) launch_change<240>(m, c, s);
-    else launch_change<kChangeWords>(m, c, s);
+hipError_t launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s) {
+    return c.used() <= 48 ? launch_change<48>(m, c, s) : c.used() <= 240 ? launch_change<240>(m, c, s) : launch_change<kChangeWords>(m, c, s);
 }
 
 // where the head's keys of a token of a sequence are
@@ -125,24 +123,26 @@ __global__ __launch_bounds__(256) void read_tokens(const CacheRows p, const Cach
 
 // Launches over rows from, from + 1, ..: as many at once as 32 bits count.
 template <class F>
-static void over_rows(CacheRows p, F&& launch) {
+static hipError_t over_rows(CacheRows p, F&& launch) {
     const int size = p.f16 ? 2 : 4;
     const int64_t each = (int64_t)p.kv_heads * (p.dim * size / 16), most = std::max<int64_t>(1, 0x7f000000 / each);
     const int rows = p.rows;
-    for (int64_t from = 0; from < rows; from += most) {
+    hipError_t e = hipSuccess;
+    for (int64_t from = 0; from < rows && e == hipSuccess; from += most) {
         p.rows = (int)std::min<int64_t>(most, rows - from);
-        launch(p, dim3((unsigned)((p.rows * each + 255) / 256)), (int)from);
+        e = launch(p, (unsigned)((p.rows * each + 255) / 256), (int)from);
         p.k.p += p.rows * p.k.tok * size;
         p.v.p += p.rows * p.v.tok * size;
     }
+    return e;
 }
 
-void launch_cache_write(const CacheRows& p, hipStream_t s) {
-    over_rows(p, [&](const CacheRows& q, dim3 grid, int from) { hipLaunchKernelGGL(write_tokens, grid, dim3(256), 0, s, q, from); });
+hipError_t launch_cache_write(const CacheRows& p, hipStream_t s) {
+    return over_rows(p, [&](const CacheRows& q, unsigned blocks, int from) { return start(write_tokens, blocks, s, q, from); });
 }
 
-void launch_cache_read(const CacheRows& p, const CacheRead& r, hipStream_t s) {
-    over_rows(p, [&](const CacheRows& q, dim3 grid, int from) { hipLaunchKernelGGL(read_tokens, grid, dim3(256), 0, s, q, r, from); });
+hipError_t launch_cache_read(const CacheRows& p, const CacheRead& r, hipStream_t s) {
+    return over_rows(p, [&](const CacheRows& q, unsigned blocks, int from) { return start(read_tokens, blocks, s, q, r, from); });
 }
 
 }  // namespace fynhip

@@ -38,8 +38,11 @@ struct Error : public std::runtime_error {
 #define FYN_HIP(call)                                                                              \
     do {                                                                                           \
         hipError_t e_ = (call);                                                                    \
-        if (e_ != hipSuccess) ::fynhip::fail(FYN_ERR_DEVICE, "%s failed: %s (%s:%d)", #call,       \
-                                             hipGetErrorString(e_), __FILE__, __LINE__);           \
+        if (e_ != hipSuccess) {                                                                    \
+            (void)hipGetLastError(); /* reported here: no later call shall find it */              \
+            ::fynhip::fail(FYN_ERR_DEVICE, "%s failed: %s (%s:%d)", #call, hipGetErrorString(e_),  \
+                           __FILE__, __LINE__);                                                    \
+        }                                                                                          \
     } while (0)
 
 struct Tensor {

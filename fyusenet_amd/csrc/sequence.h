@@ -4,9 +4,23 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 namespace fynhip {
 
 constexpr int kMaxHeadDim = 256;
+
+// One launch, with its own result.  (The thread's last error may be that of an earlier call of somebody else's, and stays what it is.)
+template <class... P, class... A>
+inline hipError_t start(void (*kernel)(P...), unsigned blocks, hipStream_t s, const A&... a) {
+    std::tuple<P...> given(a...);
+    return std::apply([&](auto&... x) {
+        void* at[] = {const_cast<void*>(static_cast<const void*>(&x))...};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(blocks), dim3(256), at, 0, s);
+        if (e != hipSuccess) (void)hipGetLastError();
+        return e;
+    }, given);
+}
 
 // Rows of a tensor [sequence, token, head, dim], distances in elements; dim is dense.
 struct SeqRows {
@@ -86,7 +100,7 @@ struct CacheMemory {
     char* pool;
     int64_t page_bytes;
 };
-void launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s);
+hipError_t launch_cache_change(const CacheMemory& m, const CacheChange& c, hipStream_t s);
 
 struct CacheRows {          // tokens between a cache and tensors
     SeqRows k, v;
@@ -94,12 +108,12 @@ struct CacheRows {          // tokens between a cache and tensors
     CacheWords words;
     int rows, kv_heads, dim, f16;
 };
-void launch_cache_write(const CacheRows& p, hipStream_t s);
+hipError_t launch_cache_write(const CacheRows& p, hipStream_t s);
 constexpr int kReadSequences = 400;
 struct CacheRead {
     int n;
     int sequence[kReadSequences], first[kReadSequences + 1];   // rows of the tensors, of this launch
 };
-void launch_cache_read(const CacheRows& p, const CacheRead& r, hipStream_t s);
+hipError_t launch_cache_read(const CacheRows& p, const CacheRead& r, hipStream_t s);
 
 }  // namespace fynhip
