@@ -120,6 +120,9 @@ static const fyn_cache_desc& checked(const fyn_cache_desc& d) {
     if (d.pages < 1 || d.sequences < 1 || d.sequences > (1 << 20)) fail(FYN_ERR_INVALID, "cache: %d pages, %d sequences", d.pages, d.sequences);
     if ((int64_t)d.pages * d.page_tokens > 0x7fffffff - 65536) fail(FYN_ERR_INVALID, "cache: %d pages of %d tokens hold more tokens than can be counted", d.pages, d.page_tokens);
     if (d.most_tokens < 0 || d.most_tokens > d.pages * d.page_tokens) fail(FYN_ERR_INVALID, "cache: sequences of up to %d tokens do not fit into %d pages", d.most_tokens, d.pages);
+    // (a page has up to 2^53 bytes)
+    const int64_t page_bytes = (int64_t)d.layers * 2 * d.kv_heads * d.page_tokens * d.head_dim * (d.storage == FYN_STORAGE_F16 ? 2 : 4);
+    if (page_bytes > (INT64_MAX >> 2) / d.pages) fail(FYN_ERR_INVALID, "cache: %d pages of %lld bytes are more than can be addressed", d.pages, (long long)page_bytes);
     const int64_t pitch = (d.most_tokens ? d.most_tokens + d.page_tokens - 1 : d.pages * d.page_tokens) / d.page_tokens;
     if (pitch * d.sequences > (1 << 30)) fail(FYN_ERR_INVALID, "cache: lists of %lld pages for each of %d sequences; give the most tokens of one (most_tokens)", (long long)pitch, d.sequences);
     return d;
