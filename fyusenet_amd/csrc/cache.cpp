@@ -66,7 +66,7 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     check_storage(a.storage);
     check_heads(a.heads, a.kv_heads, a.head_dim);
     check_sight(a.window, a.sinks, a.scale);
-    if (a.batch < 0 || a.tokens < 0 || (int64_t)a.batch * a.tokens > 0x7fffffff) fail(FYN_ERR_INVALID, "attention: %d sequences of %d tokens", a.batch, a.tokens);
+    if (a.batch < 0 || a.tokens < 0 || (int64_t)a.batch * a.tokens > 0x7fffffff - 65536) fail(FYN_ERR_INVALID, "attention: %d sequences of %d tokens", a.batch, a.tokens);
     if (a.batch == 0 || a.tokens == 0) return false;
     const int f16 = a.storage == FYN_STORAGE_F16;
     device = check_rows("queries", a.queries, f16);

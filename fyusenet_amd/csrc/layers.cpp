@@ -654,7 +654,7 @@ class AttentionLayer : public Layer {
         for (int i = 0; i < 3; i++)
             if (d.inputs[i].padding < 0) fail(FYN_ERR_INVALID, "layer %s: negative padding", d.name);
         if (!at.rows_are_sequences && padded()) fail(FYN_ERR_UNSUPPORTED, "attention layer %s: padding is supported where rows are sequences", d.name);
-        if ((int64_t)d.height * d.width > 0x7fffffff) fail(FYN_ERR_INVALID, "attention layer %s: %dx%d positions", d.name, d.width, d.height);
+        if ((int64_t)d.height * d.width > 0x7fffffff - 65536) fail(FYN_ERR_INVALID, "attention layer %s: %dx%d positions", d.name, d.width, d.height);
         oc = d.out_channels;
         oh = d.height;
         ow = d.width;

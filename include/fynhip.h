@@ -333,7 +333,7 @@ typedef struct fyn_rows {
 
 /* Every token of a padded batch over its own sequence.  lengths: device memory, `batch` numbers of tokens (read when the
  * work runs, and taken as within 0 and `tokens`), or NULL: all have `tokens`.  Rows of the result behind a sequence's length are zero.  head_dim: a
- * multiple of 8 up to 256.  scale: of the scores, 0 is 1/sqrt(head_dim).  The result must not overlap the other tensors. */
+ * multiple of 8 up to 256.  scale: of the scores, 0 is 1/sqrt(head_dim).  batch * tokens: up to 2^31 - 65537.  The result must not overlap the other tensors. */
 typedef struct fyn_attention_desc {
     uint32_t struct_size;
     int32_t storage; /* fyn_storage */
