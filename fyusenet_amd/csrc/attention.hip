@@ -8,6 +8,8 @@
 // values; where m grows both are multiplied with exp(m_old - m_new).  All of that is held in 32 bits.
 #include "attention_common.h"
 
+#include <algorithm>
+
 namespace fynhip {
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     const int columns = together ? p.common_tiles : p.tiles * p.batch, parts = together ? p.common_parts : p.parts - (BRANCHES ? p.common_parts : 0);
     const int id = (int)blockIdx.x - (together ? 0 : common_blocks), x = (id / (8 * columns)) * 8 + id % 8, col_tile = id / 8 % columns;
     if (x >= across * parts) return;
-    const int part = x / across, who = x % across, b = together ? 0 : col_tile / p.tiles, tile = together ? 0 : col_tile % p.tiles;
+    const int part = x / across, who = x % across, b = together ? 0 : p.first_batch + col_tile / p.tiles, tile = together ? 0 : col_tile % p.tiles;
     const int kv_head = BY_TOKEN ? who / group : who;
 
     const Batched in = batched<PAGED>(p, b);
@@ -486,12 +488,14 @@ static hipError_t launch_steps(const AttnParams& p, unsigned blocks, hipStream_t
 
 int attention_step(int f16, int dim) { return !f16 && dim > 128 ? 16 : 32; }
 
-int launch_attention(const AttnParams& p, hipStream_t s) {
-    if (p.tiled) return p.f16 ? launch_tiles_f16(p, s) : launch_tiles_f32(p, s);
+static int64_t steps_blocks(const AttnParams& p) {
     const int64_t across = p.by_token ? p.heads : p.kv_heads;
-    const int64_t blocks = (across * (p.parts - p.common_parts) + 7) / 8 * 8 * (int64_t)p.tiles * p.batch + (across * p.common_parts + 7) / 8 * 8 * (int64_t)p.common_tiles;
+    return (across * (p.parts - p.common_parts) + 7) / 8 * 8 * (int64_t)p.tiles * p.batch + (across * p.common_parts + 7) / 8 * 8 * (int64_t)p.common_tiles;
+}
+
+static int launch_once(const AttnParams& p, int64_t blocks, hipStream_t s) {
     if (blocks <= 0) return 0;
-    if (blocks > 0x7fffffff) return -2;
+    if (p.tiled) return p.f16 ? launch_tiles_f16(p, (unsigned)blocks, s) : launch_tiles_f32(p, (unsigned)blocks, s);
     hipError_t e;
 #define FYN_ATTN(T, D) e = launch_steps<T, D>(p, (unsigned)blocks, s)
     if (p.f16) {
@@ -509,6 +513,21 @@ int launch_attention(const AttnParams& p, hipStream_t s) {
     }
 #undef FYN_ATTN
     return e == hipSuccess ? 0 : -1;
+}
+
+int launch_attention(const AttnParams& p, hipStream_t s) {
+    // A launch has fewer than 2^32 threads: the batch in pieces where it would have more.
+    constexpr int64_t kMost = 0xffffff;
+    auto blocks = [](const AttnParams& q) { return q.tiled ? ((int64_t)q.batch * q.heads + 7) / 8 * 8 * q.tiles : steps_blocks(q); };
+    AttnParams q = p;
+    while (q.batch > 1 && blocks(q) > kMost) q.batch = (q.batch + 1) / 2;
+    if (blocks(q) > kMost || (q.batch < p.batch && p.parts > 1)) return -2;   // (rows in parts are few)
+    for (const int each = q.batch; q.first_batch < p.batch; q.first_batch += each) {
+        q.batch = std::min(each, p.batch - q.first_batch);
+        const int rc = launch_once(q, blocks(q), s);
+        if (rc != 0) return rc;
+    }
+    return 0;
 }
 
 }  // namespace fynhip

@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
     const int units = p.batch * p.heads, rounds = (units + 7) / 8, id = blockIdx.x;
     const int unit = id / 8 % rounds * 8 + id % 8, tile = p.tiles - 1 - id / 8 / rounds;
     if (unit >= units) return;
-    const int b = unit / p.heads, kv_head = unit % p.heads % p.kv_heads, head = kv_head * (p.heads / p.kv_heads) + unit % p.heads / p.kv_heads;
+    const int b = p.first_batch + unit / p.heads, kv_head = unit % p.heads % p.kv_heads, head = kv_head * (p.heads / p.kv_heads) + unit % p.heads / p.kv_heads;
     const Batched in = batched<PAGED>(p, b);
     if (tile * QUERIES >= in.count) return;
     const int seen_rows = PAGED ? in.count : min(in.count, in.len);   // (padded rows see nothing)
@@ -422,23 +422,20 @@ typedef float Stored;
 #endif
 
 template <int QW>
-static int launch_class(const AttnParams& p, hipStream_t s) {
-    const int64_t blocks = ((int64_t)p.batch * p.heads + 7) / 8 * 8 * p.tiles;
-    if (blocks <= 0) return 0;
-    if (blocks > 0x7fffffff) return -2;
+static int launch_class(const AttnParams& p, unsigned blocks, hipStream_t s) {
     hipError_t e;
-    if (p.dim <= 32) e = launch_tiles<Stored, 32, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 64) e = launch_tiles<Stored, 64, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 96) e = launch_tiles<Stored, 96, QW>(p, (unsigned)blocks, s);
-    else if (p.dim <= 128) e = launch_tiles<Stored, 128, QW>(p, (unsigned)blocks, s);
+    if (p.dim <= 32) e = launch_tiles<Stored, 32, QW>(p, blocks, s);
+    else if (p.dim <= 64) e = launch_tiles<Stored, 64, QW>(p, blocks, s);
+    else if (p.dim <= 96) e = launch_tiles<Stored, 96, QW>(p, blocks, s);
+    else if (p.dim <= 128) e = launch_tiles<Stored, 128, QW>(p, blocks, s);
 #if FYN_ATTN_HALF
-    else e = launch_tiles<Stored, 256, QW>(p, (unsigned)blocks, s);
+    else e = launch_tiles<Stored, 256, QW>(p, blocks, s);
 #else
     else return -1;   // (queries and sums of 32 bits: more registers than a wave has)
 #endif
     return e == hipSuccess ? 0 : -1;
 }
 
-int FYN_ATTN_NAME(const AttnParams& p, hipStream_t s) { return p.tiled == 128 ? launch_class<4>(p, s) : launch_class<2>(p, s); }
+int FYN_ATTN_NAME(const AttnParams& p, unsigned blocks, hipStream_t s) { return p.tiled == 128 ? launch_class<4>(p, blocks, s) : launch_class<2>(p, blocks, s); }
 
 }  // namespace fynhip

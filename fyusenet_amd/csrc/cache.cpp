@@ -98,7 +98,7 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
 
 void run_attention(const AttnParams& p, hipStream_t s) {
     const int rc = launch_attention(p, s);
-    if (rc == -2) fail(FYN_ERR_INVALID, "attention: more heads and tokens than one launch takes");
+    if (rc == -2) fail(FYN_ERR_INVALID, "attention: more heads and tokens of one sequence than a launch takes");
     if (rc != 0) fail(FYN_ERR_DEVICE, "attention: launch failed");
 }
 

@@ -54,6 +54,7 @@ struct AttnParams {
     CacheWords words;
     const int* lengths;     // nothing paged: tokens of each sequence, or null
     int paged, f16;
+    int first_batch;        // of one launch: the sequences [first_batch, first_batch + batch) of the batch
     int batch, tokens;      // nothing paged: rows of each sequence; paged: rows of q in all
     int heads, kv_heads, dim;
     int causal, window, sinks;
@@ -73,10 +74,10 @@ struct AttnParams {
     float* part_ml;         // ... [2]: maximum and sum
 };
 
-// 0, -1 where the launch failed, -2 where it would have more workgroups than there can be.
+// 0, -1 where a launch failed, -2 where one sequence would have more workgroups than a launch can.
 int launch_attention(const AttnParams& p, hipStream_t s);
-int launch_tiles_f16(const AttnParams& p, hipStream_t s);   // (called by it)
-int launch_tiles_f32(const AttnParams& p, hipStream_t s);   // ... up to 128 dims
+int launch_tiles_f16(const AttnParams& p, unsigned blocks, hipStream_t s);   // (called by it)
+int launch_tiles_f32(const AttnParams& p, unsigned blocks, hipStream_t s);   // ... up to 128 dims
 int attention_step(int f16, int dim);   // keys of one step of the kernel (AttnParams::chunk counts them)
 
 // What the host changes of a cache in one launch.  It travels as the kernel's argument (at most 4 KB, and 256 bytes where it is

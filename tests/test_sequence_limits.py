@@ -25,3 +25,43 @@ def test_attention_refuses_more_tokens_than_can_be_counted():
         with pytest.raises(fa.FynException) as e:
             capi.check(capi.lib().fyn_attention(ctypes.byref(d), None))
         assert e.value.code == capi.ERR_INVALID and "%d sequences of %d tokens" % (batch, tokens) in str(e.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,tokens,heads,kv_heads", [(300000, 1, 64, 8), (530000, 2, 32, 32)])
+def test_more_sequences_than_a_launch_takes(batch, tokens, heads, kv_heads):
+    """Nineteen and seventeen million workgroups; a launch has fewer than 2^32 threads."""
+    torch = pytest.importorskip("torch")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(batch, tokens, h, 8, generator=gen, device="cuda", dtype=torch.float16) for h in (heads, kv_heads, kv_heads))
+    out = torch.full_like(q, 9.0)
+    fa.attention(q, k, v, out, causal=True, stream=torch.cuda.current_stream().cuda_stream)
+    # a sequence's first token sees itself alone
+    assert torch.equal(out[:, 0], v[:, 0].repeat_interleave(heads // kv_heads, 1))
+    if tokens > 1:
+        s = [(q[:, 1].float() * k[:, j].float()).sum(-1) / 8 ** 0.5 for j in (0, 1)]
+        w = torch.sigmoid(s[1] - s[0])[..., None]
+        want = (1 - w) * v[:, 0].float() + w * v[:, 1].float()
+        # (the weights to 2^-17 or so, and the result's rounding)
+        assert ((out[:, 1].float() - want).abs() <= 2.0 ** -14 + 2.0 ** -11 * want.abs()).all()
+
+
+@pytest.mark.gpu
+def test_more_sequences_of_a_cache_than_a_launch_takes():
+    torch = pytest.importorskip("torch")
+    n, heads = 70000, 256
+    s = torch.cuda.current_stream().cuda_stream
+    cache = fa.SequenceCache(fa.STORAGE_F16, 1, heads, heads, 8, 8, n, n, 8)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(n, heads, 8, generator=gen, device="cuda", dtype=torch.float16) for _ in range(3))
+    out = torch.full_like(q, 9.0)
+    who = list(range(n))
+    cache.extend(who, [1] * n, stream=s)
+    cache.write(0, k, v, stream=s)
+    cache.attend(0, q, out, stream=s)
+    assert torch.equal(out, v)
+    cache.extend(who[::-1], [1] * n, stream=s)      # (each has itself and one before: the same value twice)
+    cache.write(0, q.flip(0), v.flip(0), stream=s)
+    cache.attend(0, q.flip(0), out, stream=s)
+    assert ((out.float() - v.flip(0).float()).abs() <= 2.0 ** -11 * v.flip(0).float().abs() + 2.0 ** -24).all()
+    cache.close()
