@@ -562,8 +562,8 @@ class AttentionLayerBuilder(GPULayerBuilder):
             d.inputs[i].channels, d.inputs[i].padding, d.inputs[i].flags = n * self.headDim_, self.inputPadding_, 0
 
     def attention(self):
-        return capi.AttentionLayer(capi.ctypes.sizeof(capi.AttentionLayer), self.heads_, self.kvHeads_, int(self.causal_), self.window_, self.sinks_,
-                                   int(self.rows_), self.scale_)
+        return capi.AttentionLayer(capi.ctypes.sizeof(capi.AttentionLayer), *map(capi.int32, (self.heads_, self.kvHeads_, int(self.causal_), self.window_, self.sinks_,
+                                                                                               int(self.rows_))), self.scale_)
 
 
 class CustomLayerBuilder(GPULayerBuilder):

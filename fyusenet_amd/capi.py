@@ -90,6 +90,13 @@ class CustomLayer(ctypes.Structure):
     _fields_ = [("user", ctypes.c_void_p), ("setup", CUSTOM_SETUP_FN), ("forward", CUSTOM_FORWARD_FN), ("cleanup", CUSTOM_CLEANUP_FN)]
 
 
+def int32(x):
+    """A number that a struct or an argument of 32 bits holds.  (ctypes takes the last 32 bits of any other.)"""
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise FynException(ERR_INVALID, "%s is not within 32 bits" % x)
+    return x
+
+
 class Rows(ctypes.Structure):
     """struct fyn_rows."""
     _fields_ = [("data", ctypes.c_void_p), ("sequence_pitch", ctypes.c_int64), ("token_pitch", ctypes.c_int64), ("head_pitch", ctypes.c_int64)]

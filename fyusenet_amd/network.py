@@ -83,7 +83,7 @@ class Layer:
 
     def bindCache(self, cache, cacheLayer=0):
         """fyn_layer_bind_cache: an attention layer works on a SequenceCache from now on (None: no longer)."""
-        capi.check(capi.lib().fyn_layer_bind_cache(self._net._h, self.number, cache._h if cache is not None else None, cacheLayer))
+        capi.check(capi.lib().fyn_layer_bind_cache(self._net._h, self.number, cache._h if cache is not None else None, capi.int32(cacheLayer)))
 
     def timeKernel(self, iters):
         ms = ctypes.c_float(0)

@@ -4,6 +4,7 @@ Tensors are device memory of the caller's: anything with data_ptr(), dtype, shap
 with __cuda_array_interface__, a capi.TensorView as custom layers get them, or a DeviceArray.  `stream` is a hipStream_t as
 an integer (torch.cuda.current_stream().cuda_stream), 0 the default stream.  Calls return before the work is done.
 """
+import array
 import ctypes
 import struct
 
@@ -138,15 +139,13 @@ def attention(queries, keys, values, result, lengths=None, causal=True, window=0
         capi.check(status)
 
 
-_arrays = {}
-
-
 def _ints(v):
-    n = len(v)
-    t = _arrays.get(n)
-    if t is None:
-        t = _arrays[n] = ctypes.c_int32 * n
-    return t(*v)
+    """int32 values as a call's argument.  (ctypes by itself takes any integer, and its last 32 bits.)"""
+    try:
+        a = array.array("i", v)
+    except (OverflowError, TypeError) as e:
+        raise capi.FynException(capi.ERR_INVALID, "int32 values are expected: %s" % e)
+    return (ctypes.c_int32 * len(a)).from_buffer(a)
 
 
 class SequenceCache:
@@ -159,8 +158,8 @@ class SequenceCache:
 
     def __init__(self, storage, layers, heads, kv_heads, head_dim, page_tokens, pages, sequences, most_tokens=0, device=0):
         self._h = ctypes.c_void_p()
-        d = capi.CacheDesc(ctypes.sizeof(capi.CacheDesc), storage, layers, heads, kv_heads, head_dim, page_tokens, pages, sequences, most_tokens)
-        capi.check(capi.lib().fyn_cache_create(device, ctypes.byref(d), ctypes.byref(self._h)))
+        d = capi.CacheDesc(ctypes.sizeof(capi.CacheDesc), *map(capi.int32, (storage, layers, heads, kv_heads, head_dim, page_tokens, pages, sequences, most_tokens)))
+        capi.check(capi.lib().fyn_cache_create(capi.int32(device), ctypes.byref(d), ctypes.byref(self._h)))
         self.storage, self.layers, self.heads, self.kv_heads, self.head_dim = storage, layers, heads, kv_heads, head_dim
         self.page_tokens, self.sequences = page_tokens, sequences
         self._type = _TYPES[storage]
@@ -180,7 +179,7 @@ class SequenceCache:
 
     def write(self, layer, keys, values, stream=0):
         k, v, rows = self._kv(keys, values)
-        capi.check(_call("fyn_cache_write", _V, ctypes.c_int, _V, _V, ctypes.c_int, _V)(self._h, layer, k, v, rows, stream))
+        capi.check(_call("fyn_cache_write", _V, ctypes.c_int, _V, _V, ctypes.c_int, _V)(self._h, capi.int32(layer), k, v, capi.int32(rows), stream))
 
     def attend(self, layer, queries, result, window=0, sinks=0, scale=0.0, stream=0):
         q = _take(queries, "queries")
@@ -190,7 +189,7 @@ class SequenceCache:
                              *_rows(_take(result, "result"), "result", self._type, shape))
         except (struct.error, OverflowError) as e:
             raise capi.FynException(capi.ERR_INVALID, "attend: %s" % e)
-        status = _call("fyn_cache_attend", _V, ctypes.c_int, _V, _V)(self._h, layer, d, stream)
+        status = _call("fyn_cache_attend", _V, ctypes.c_int, _V, _V)(self._h, capi.int32(layer), d, stream)
         if status:
             capi.check(status)
 
@@ -198,10 +197,10 @@ class SequenceCache:
         """Keys and values of whole sequences into [tokens of all of them, kv_heads, dim]."""
         k, v, rows = self._kv(keys, values)
         capi.check(_call("fyn_cache_read", _V, ctypes.c_int, _V, ctypes.c_int, _V, _V, ctypes.c_int, _V)(
-            self._h, len(sequences), _ints(sequences), layer, k, v, rows, stream))
+            self._h, len(sequences), _ints(sequences), capi.int32(layer), k, v, capi.int32(rows), stream))
 
     def fork(self, source, targets, tokens=-1, stream=0):
-        capi.check(capi.lib().fyn_cache_fork(self._h, source, len(targets), _ints(targets), tokens, stream))
+        capi.check(capi.lib().fyn_cache_fork(self._h, capi.int32(source), len(targets), _ints(targets), capi.int32(tokens), stream))
 
     def copy(self, sources, targets, stream=0):
         self._same(sources, targets, "copy")

@@ -65,3 +65,24 @@ def test_more_sequences_of_a_cache_than_a_launch_takes():
     cache.attend(0, q.flip(0), out, stream=s)
     assert ((out.float() - v.flip(0).float()).abs() <= 2.0 ** -11 * v.flip(0).float().abs() + 2.0 ** -24).all()
     cache.close()
+
+
+class _Unopened(fa.SequenceCache):
+    """The Python side of a cache whose handle is null: what it refuses by itself."""
+
+    def __init__(self):
+        self._h, self.kv_heads, self.head_dim, self.heads, self._type = ctypes.c_void_p(), 1, 8, 1, "float16"
+
+
+@pytest.mark.parametrize("far", [2 ** 32, 2 ** 32 + 1, 2 ** 31, -2 ** 31 - 1, 2 ** 64])
+def test_python_refuses_numbers_beyond_32_bits(far):
+    """... instead of taking their last 32 bits: sequence 2^32 is not sequence 0."""
+    c, x = _Unopened(), fa.DeviceArray(1 << 20, "float16", (3, 1, 8))
+    b = fa.AttentionLayerBuilder(1, 1, 8, "mix").window(far)
+    for call in (lambda: c.extend([far], [1]), lambda: c.extend([0], [far]), lambda: c.fork(far, [1]), lambda: c.fork(0, [far]), lambda: c.fork(0, [1], far),
+                 lambda: c.copy([0], [far]), lambda: c.truncate([0], [far]), lambda: c.free([far]), lambda: c.lengths([far]), lambda: c.write(far, x, x),
+                 lambda: c.attend(far, x, x), lambda: c.read([far], 0, x, x), lambda: c.read([0], far, x, x), b.attention,
+                 lambda: fa.SequenceCache(fa.STORAGE_F16, 1, 1, 1, 8, 8, far, 1), lambda: fa.SequenceCache(fa.STORAGE_F16, 1, 1, 1, 8, 8, 1, 1, far)):
+        with pytest.raises(fa.FynException) as e:
+            call()
+        assert e.value.code == capi.ERR_INVALID and "null" not in str(e.value) and "cache:" not in str(e.value)
