@@ -109,13 +109,13 @@ class PageBook {
     }
 
     // The first `tokens` tokens of a sequence (-1: all) become those of empty ones too, in the same pages.  The words of
-    // the lists are not noted as changed: the rows are copies of the source's (fork_words() of them).
+    // the lists are not noted as changed: the rows are copies of the source's, as long as the list of a branch is.
     void fork(int source, int n, const int* targets, int tokens) {
         check(1, &source, "fork");
         check(n, targets, "fork");
         const int len = words[source];
-        if (tokens < 0) tokens = len;
-        if (tokens > len) refuse(false, "sequence " + std::to_string(source) + " has " + std::to_string(len) + " tokens, not " + std::to_string(tokens));
+        if (tokens == -1) tokens = len;
+        if (tokens < 0 || tokens > len) refuse(false, "sequence " + std::to_string(source) + " has " + std::to_string(len) + " tokens, not " + std::to_string(tokens));
         for (int i = 0; i < n; i++) {
             if (targets[i] == source) refuse(false, "a sequence cannot become a branch of itself");
             empty(targets[i]);
