@@ -1,7 +1,9 @@
 // Host side of attention and of the cache of keys and values: checks, launches, order between streams.
 #include "cache.h"
 
+#include <algorithm>
 #include <cmath>
+#include <iterator>
 
 namespace fynhip {
 
@@ -27,6 +29,18 @@ int check_rows(const char* what, const fyn_rows& r, int f16) {
         fail(FYN_ERR_INVALID, "%s: not device memory", what);
     }
     return at.device;
+}
+
+// Rows that are written: no two of them may share memory.
+static void check_apart(const char* what, const fyn_rows& r, int64_t sequences, int64_t tokens, int64_t heads, int dim) {
+    std::pair<int64_t, int64_t> axes[] = {{r.head_pitch, heads}, {r.token_pitch, tokens}, {r.sequence_pitch, sequences}};
+    std::sort(std::begin(axes), std::end(axes));
+    __int128 span = dim;   // of what the axes so far reach over
+    for (auto [pitch, n] : axes) {
+        if (n <= 1) continue;
+        if (pitch < span) fail(FYN_ERR_INVALID, "%s: rows of %d values at distances of %lld overlap", what, dim, (long long)pitch);
+        span += (__int128)(n - 1) * pitch;
+    }
 }
 
 static SeqRows rows_of(const fyn_rows& r) { return SeqRows{static_cast<char*>(r.data), r.sequence_pitch, r.token_pitch, r.head_pitch}; }
@@ -69,6 +83,7 @@ bool attention_params(const fyn_attention_desc& a, AttnParams& p, int& device) {
     if (a.batch < 0 || a.tokens < 0 || (int64_t)a.batch * a.tokens > 0x7fffffff - 65536) fail(FYN_ERR_INVALID, "attention: %d sequences of %d tokens", a.batch, a.tokens);
     if (a.batch == 0 || a.tokens == 0) return false;
     const int f16 = a.storage == FYN_STORAGE_F16;
+    check_apart("result", a.result, a.batch, a.tokens, a.heads, a.head_dim);
     device = check_rows("queries", a.queries, f16);
     if (check_rows("keys", a.keys, f16) != device || check_rows("values", a.values, f16) != device || check_rows("result", a.result, f16) != device)
         fail(FYN_ERR_INVALID, "attention: the tensors are on different devices");
@@ -379,6 +394,8 @@ void Cache::read(int n, const int* seqs, int layer, const fyn_rows& k, const fyn
     }
     if (total != rows) fail(FYN_ERR_INVALID, "cache: the sequences have %lld tokens, the tensors %d", (long long)total, rows);
     if (rows == 0) return;
+    check_apart("keys", k, 1, rows, d.kv_heads, d.head_dim);
+    check_apart("values", v, 1, rows, d.kv_heads, d.head_dim);
     if (check_rows("keys", k, f16) != device || check_rows("values", v, f16) != device) fail(FYN_ERR_INVALID, "cache: keys or values are on another device");
     OnDevice on(device);
     settle(s);   // (which rows there are is settled on the host)
@@ -424,6 +441,7 @@ void Cache::attend(int layer, const fyn_attend_desc& a, hipStream_t s) {
     check_sight(a.window, a.sinks, a.scale);
     if (a.rows != book_.batch_rows()) fail(FYN_ERR_INVALID, "cache: the batch has %d new tokens, the tensors %d", book_.batch_rows(), a.rows);
     if (a.rows == 0) return;
+    check_apart("result", a.result, 1, a.rows, d.heads, d.head_dim);
     if (check_rows("queries", a.queries, f16) != device || check_rows("result", a.result, f16) != device) fail(FYN_ERR_INVALID, "cache: queries or result are on another device");
     OnDevice on(device);
     const bool captured = enter(s);

@@ -324,7 +324,8 @@ int fyn_layer_kernel_info(fyn_net* net, int layer, char* buf, size_t buflen);
  * h / (heads / kv_heads). */
 
 /* Rows of a tensor: element (sequence, token, head, x) is at sequence*sequence_pitch + token*token_pitch + head*head_pitch + x,
- * in elements of the storage type.  Address and pitches are multiples of 16 bytes.  The cache's calls take tokens of all
+ * in elements of the storage type.  Address and pitches are multiples of 16 bytes; rows that are read may be the same ones (a
+ * pitch of 0), rows that are written may not overlap.  The cache's calls take tokens of all
  * sequences of a batch one behind the other and do not look at sequence_pitch. */
 typedef struct fyn_rows {
     void* data;

@@ -86,3 +86,37 @@ def test_python_refuses_numbers_beyond_32_bits(far):
         with pytest.raises(fa.FynException) as e:
             call()
         assert e.value.code == capi.ERR_INVALID and "null" not in str(e.value) and "cache:" not in str(e.value)
+
+
+#   shape [batch, tokens, heads, 8], strides
+OVERLAPPING = [((2, 3, 4, 8), (0, 32, 8, 1)), ((2, 3, 4, 8), (96, 0, 8, 1)), ((2, 3, 4, 8), (96, 32, 0, 1)), ((2, 3, 4, 8), (96, 24, 8, 1)), ((2, 3, 4, 8), (88, 32, 8, 1)),
+               ((1, 3, 1, 8), (0, 0, 0, 1))]
+APART = [((2, 3, 4, 8), (96, 32, 8, 1)), ((2, 3, 4, 8), (8, 64, 16, 1)), ((2, 3, 4, 8), (96, 8, 24, 1)), ((1, 3, 1, 8), (0, 16, 0, 1)), ((1, 1, 1, 8), (0, 0, 0, 1))]
+
+
+@pytest.mark.parametrize("shape,strides", OVERLAPPING + APART)
+def test_results_that_overlap_are_refused(shape, strides):
+    """(The addresses here are nobody's: what is refused for its rows is refused in front of that.)"""
+    q = fa.DeviceArray(1 << 20, "float16", shape)
+    with pytest.raises(fa.FynException) as e:
+        fa.attention(q, q, q, fa.DeviceArray(1 << 24, "float16", shape, strides))
+    assert e.value.code == capi.ERR_INVALID and ("overlap" in str(e.value)) == ((shape, strides) in OVERLAPPING)
+
+
+@pytest.mark.gpu
+def test_results_of_a_cache_that_overlap_are_refused():
+    torch = pytest.importorskip("torch")
+    s = torch.cuda.current_stream().cuda_stream
+    c = fa.SequenceCache(fa.STORAGE_F16, 1, 4, 2, 8, 8, 4, 2)
+    kv, q = torch.ones(3, 2, 8, dtype=torch.float16, device="cuda"), torch.ones(3, 4, 8, dtype=torch.float16, device="cuda")
+    c.extend([0], [3], stream=s)
+    c.write(0, kv[:1].expand(3, 2, 8), kv[:, :1].expand(3, 2, 8), stream=s)     # (what is read may be the same for all)
+    out, back = torch.zeros_like(q), torch.zeros_like(kv)
+    for call in (lambda: c.attend(0, q, out[:1].expand(3, 4, 8)), lambda: c.attend(0, q, out[:, :1].expand(3, 4, 8)),
+                 lambda: c.read([0], 0, back[:1].expand(3, 2, 8), torch.zeros_like(kv)), lambda: c.read([0], 0, torch.zeros_like(kv), back[:, :1].expand(3, 2, 8))):
+        with pytest.raises(fa.FynException) as e:
+            call()
+        assert "overlap" in str(e.value)
+    c.attend(0, q[:1].expand(3, 4, 8), out, stream=s)
+    c.read([0], 0, back, torch.zeros_like(kv), stream=s)
+    assert (out == 1).all() and (back == 1).all()
