@@ -222,7 +222,8 @@ void Cache::settle(hipStream_t s) {
 void Cache::order(hipStream_t s) {
     std::lock_guard<std::mutex> lock(mu_);
     OnDevice on(device);
-    enter(s);
+    if (capturing(s)) fail(FYN_ERR_STATE, "cache: a stream that is being captured is not put in order (the stream that replays is, in front of the replay)");
+    join_streams(s);
 }
 
 std::vector<int> Cache::expect(int rows, hipStream_t s) {

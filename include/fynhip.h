@@ -408,7 +408,8 @@ int fyn_net_add_attention_layer(fyn_net* net, const fyn_layer_desc* desc, const 
  * (as the cache's layer `cache_layer`) before it attends to the cache.  fyn_cache_extend comes before each pass;
  * a pass is refused where the batch has not as many new tokens as the layer has positions.  The ports have no padding.  cache NULL: the layer is as described again. */
 int fyn_layer_bind_cache(fyn_net* net, int layer, fyn_cache* cache, int cache_layer);
-/* What this cache's calls have queued so far comes before what is queued on this stream from now on. */
+/* What this cache's calls have queued so far comes before what is queued on this stream from now on, and that before what later calls of
+ * the cache on other streams do: in front of a replay, which is none of the cache's calls.  Not under stream capture. */
 int fyn_cache_order(fyn_cache* cache, void* hip_stream);
 
 #ifdef __cplusplus

@@ -4,6 +4,8 @@ import pytest
 
 import fyusenet_amd as fa
 from fyusenet_amd import capi
+from tests.test_gpu_sequences import close
+from tests.test_gpu_sequences_precision import exact
 from tests.util import make_single_layer_net
 
 torch = pytest.importorskip("torch")
@@ -61,3 +63,47 @@ def test_timing_a_layer_waits_for_the_cache(storage):
     net.layers[1].bindCache(None)
     assert net.layers[1].timeKernel(3) > 0
     net.cleanup()
+
+
+@pytest.mark.gpu
+def test_replays_in_order():
+    """A captured step on a stream of its own, put in order by fyn_cache_order in front of each replay, between calls on others; under capture
+    there is no order to be had, and that is said."""
+    heads, kv, dim, n = 4, 2, 64, 3
+    cache = fa.SequenceCache(fa.STORAGE_F16, 1, heads, kv, dim, 16, 400, n)
+    gen = torch.Generator().manual_seed(3)
+    k, v, q = (torch.randn(n, h, dim, generator=gen).half().cuda() for h in (kv, kv, heads))
+    out, side, mine = torch.zeros_like(q), torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    old = [torch.randn(n * 100, kv, dim, generator=gen).half().cuda() for _ in range(2)]
+    torch.cuda.synchronize()
+    cache.extend([0, 1, 2], [100] * n, stream=side.cuda_stream)
+    cache.write(0, *old, stream=side.cuda_stream)
+    have = [[x[s * 100:(s + 1) * 100] for x in old] for s in range(n)]
+    cache.extend([0, 1, 2], [1] * n, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=mine):
+        cache.write(0, k, v, stream=mine.cuda_stream)
+        cache.attend(0, q, out, stream=mine.cuda_stream)
+        with pytest.raises(fa.FynException) as e:
+            cache.order(mine.cuda_stream)
+        assert e.value.code == capi.ERR_STATE
+    for turn in range(4):
+        if turn:
+            behind_something_long(side)
+            cache.extend([0, 1, 2], [1] * n, stream=side.cuda_stream)
+        cache.order(mine.cuda_stream)
+        with torch.cuda.stream(mine):
+            graph.replay()
+        rows = sum(cache.lengths([0, 1, 2]))
+        have = [[torch.cat([x, y[s:s + 1]]) for x, y in zip(have[s], (k, v))] for s in range(n)]
+        got = [torch.empty(rows, kv, dim, dtype=torch.float16, device="cuda") for _ in range(2)]
+        torch.cuda.current_stream().synchronize()
+        cache.read([0, 1, 2], 0, *got, stream=side.cuda_stream)    # (behind the replay)
+        cache.order(torch.cuda.current_stream().cuda_stream)
+        for i, x in enumerate(got):
+            assert torch.equal(x, torch.cat([have[s][i] for s in range(n)]))
+        for s in range(n):
+            close(out[s:s + 1], *exact(q[s:s + 1], *have[s], have[s][0].shape[0] - 1, 100))
+        torch.cuda.synchronize()
