@@ -178,7 +178,6 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     VVec v[S::TILES][4][S::BLOCKS];
     // Pieces behind a head's last value are taken from within it.  Of the values they end in dims that nobody stores; of the keys they are
     // zero in the product, as the queries are (zero times an infinity of the head's own would not be).
-    auto has_piece = [&](int s) { return (s + 1) * 4 * S::VEC <= S::LEAST || (s * 4 + g) * S::VEC < p.dim; };
     auto load_keys = [&](const Where& w) {
 #pragma unroll
         for (int t = 0; t < S::TILES; t++)
@@ -210,18 +209,24 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
         const int at = at_of(st);
         const Where next = where(at_of(min(st + 4, end - 1)));
         // scores
+        if (p.dim < DIMS) {
+#pragma unroll
+            for (int s = 0; s < S::KLOADS; s++)
+#pragma unroll
+                for (int t = 0; t < S::TILES; t++)
+                    if ((s + 1) * 4 * S::VEC > S::LEAST && (s * 4 + g) * S::VEC >= p.dim) k[t][s] = KVec{};
+        }
         f4 sc[S::TILES];
 #pragma unroll
         for (int t = 0; t < S::TILES; t++) {
             sc[t] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < S::KLOADS; s++) {
-                const KVec piece = has_piece(s) ? k[t][s] : KVec{};
                 if constexpr (F16) {
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece, q[s], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], sc[t], 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[e], q[s][e], sc[t], 0, 0, 0);
+                    for (int e = 0; e < 4; e++) sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][s][e], q[s][e], sc[t], 0, 0, 0);
                 }
             }
             sc[t] *= p.scale_log2;

@@ -45,8 +45,8 @@ struct TileShape {
     static constexpr int LDS = 2 * HALF;
     static_assert(LDS + 2048 <= 160 * 1024, "a CU's LDS");
     // Weights are 2^SHIFT times as large as relative to the running maximum, which may be LAG binary orders of magnitude behind the true
-    // one.  (In 32 bits both are 0: the larger the exponent's argument is, the fewer bits it has behind the point.)
-    static constexpr float SHIFT = F16 ? 6.f : 0.f, LAG = F16 ? 8.f : 0.f;
+    // one.  (In 32 bits the exponent's argument is 1 at most: the larger it is, the fewer bits it has behind the point.)
+    static constexpr float SHIFT = F16 ? 6.f : 0.f, LAG = F16 ? 8.f : 1.f;
     static constexpr int WAVES = DIMS <= (F16 ? 128 : 64) && LDS <= 64 * 1024 ? 2 : 1;   // workgroups that share a CU (their registers)
 };
 
@@ -227,14 +227,21 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
             for (int s = 0; s < S::PIECES / 2; s++) kf[s] = *reinterpret_cast<const KVec*>(kl + 16 * row_piece<S::PITCH>(mates * 32 + c, 2 * s + half));
             if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+            // (Pieces behind the head are zero.  In 32 bits in front of the products, for heads that have such: 8 heads of 128, 4096 tokens,
+            // 763 us, and 783 with a select for each product; in 16 bits, heads of 256, 2048 tokens, the branch spills: 222 us and 160.)
+            if (!F16 && p.dim < DIMS) {
+#pragma unroll
+                for (int s = 0; s < S::PIECES / 2; s++)
+                    if ((2 * s + 2) * S::VEC > S::LEAST && (2 * s + half) * S::VEC >= p.dim) kf[s] = KVec{};
+            }
 #pragma unroll
             for (int s = 0; s < S::PIECES / 2; s++) {
-                const KVec piece = (2 * s + 2) * S::VEC <= S::LEAST || (2 * s + half) * S::VEC < p.dim ? kf[s] : KVec{};
                 if constexpr (F16) {
+                    const KVec piece = (2 * s + 2) * S::VEC <= S::LEAST || (2 * s + half) * S::VEC < p.dim ? kf[s] : KVec{};
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(piece, q[s], sc, 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[e], q[s][e], sc, 0, 0, 0);
+                    for (int e = 0; e < 4; e++) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[s][e], q[s][e], sc, 0, 0, 0);
                 }
             }
             if (!((at >= all.lo && at + 32 <= all.hi) || at + 32 <= all.first)) {
@@ -266,8 +273,8 @@ __global__ __launch_bounds__(256, (TileShape<T, DIMS, QW>::WAVES)) void attend_t
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, sc[r]);
             top = across(top) * scale;
-            // In 16 bits the sums are relative to a maximum that may be the true one's 2^-8 (with weights up to 2^14 then): it follows where
-            // a query is further off, which after the first tiles is seldom.
+            // The sums are relative to a maximum that may be the true one's 2^-LAG (in 16 bits with weights up to 2^14 then): it follows where
+            // a query is further off, which after the first tiles is seldom.  (fp32, 2 maps of 1924, 8 heads of 64: 65 us, and 68 if it always follows.)
             if (__any(top > m + S::LAG)) {
                 const float m_new = top > m + S::LAG ? top : m, alpha = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - m_new);   // (by each query alone)
                 m = m_new;
