@@ -80,7 +80,7 @@ def test_python_refuses_numbers_beyond_32_bits(far):
     c, x = _Unopened(), fa.DeviceArray(1 << 20, "float16", (3, 1, 8))
     b = fa.AttentionLayerBuilder(1, 1, 8, "mix").window(far)
     for call in (lambda: c.extend([far], [1]), lambda: c.extend([0], [far]), lambda: c.fork(far, [1]), lambda: c.fork(0, [far]), lambda: c.fork(0, [1], far),
-                 lambda: c.copy([0], [far]), lambda: c.truncate([0], [far]), lambda: c.free([far]), lambda: c.lengths([far]), lambda: c.write(far, x, x),
+                 lambda: c.copy([0], [far]), lambda: c.extend(list(range(20)) + [far], [1] * 21), lambda: c.free([3] * 12 + [far]), lambda: c.truncate([0], [far]), lambda: c.free([far]), lambda: c.lengths([far]), lambda: c.write(far, x, x),
                  lambda: c.attend(far, x, x), lambda: c.read([far], 0, x, x), lambda: c.read([0], far, x, x), b.attention,
                  lambda: fa.SequenceCache(fa.STORAGE_F16, 1, 1, 1, 8, 8, far, 1), lambda: fa.SequenceCache(fa.STORAGE_F16, 1, 1, 1, 8, 8, 1, 1, far)):
         with pytest.raises(fa.FynException) as e:
