@@ -26,9 +26,10 @@ namespace fynhip {
 //
 // Memory bound where a group's heads are the columns: every key and value is read once, in rows of 16 bytes a lane.  The next
 // step's loads are under way while a step is worked on (in the registers that its products have freed).  64 sequences of 32768
-// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 57 to 64 us
-// (4.1 to 4.6 TB/s: a workgroup's start, its joins and the unequal lengths weigh there); 16 with a window of 4096, 8 heads of 96, fp32:
-// 74 us (4.8 TB/s).  Over pages that all sequences of a batch begin with, the columns are heads of several sequences.  Sixteen tokens as columns serve short prompts: 12 heads of 197 tokens take 6.7 us, 9.0 in tiles.
+// tokens, 8 key heads of 128, fp16: 1.24 ms, 6.9 TB/s of the 7.1 that reading alone reaches; 24 ragged ones of up to 5000: 57 to 67 us
+// (3.9 to 4.6 TB/s: a workgroup's start, its joins, the unequal lengths and the parts' short rests weigh there); 16 with a window of 4096,
+// 8 heads of 96, fp32: 72 to 74 us (4.8 TB/s).  Over pages that all sequences of a batch begin with, the columns are heads of several
+// sequences.  Sixteen tokens as columns serve short prompts: 12 heads of 197 tokens take 7.1 us, 8.7 in tiles.
 // ---------------------------------------------------------------------------------------------------------------------
 template <class T, int DIMS>
 struct Shape {
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256, (Shape<T, DIMS>::WAVES)) void attend_steps(con
     if (!valid || !inside) mine.lo = mine.hi = mine.first = 0;
     const int a_steps = (any.first + S::STEP - 1) / S::STEP, b_first = max(any.lo / S::STEP, a_steps);
     const int b_steps = max(0, (any.hi + S::STEP - 1) / S::STEP - b_first), steps = a_steps + b_steps;
-    // (equal parts for every row, so that those of long and short sequences take equally long)
+    // (parts of as many steps for every row, and what is left as its last one: those of long and short sequences take equally long)
     const int chunk = max(together ? p.common_chunk : p.chunk, (steps + parts - 1) / parts), begin = part * chunk, end = min(steps, begin + chunk);
     if (begin > 0 && begin >= end) return;
     const int most = max(any.hi, any.first);   // positions from here on are not read

@@ -15,10 +15,12 @@
 //
 // In 16 bits a weight goes into the second product as two numbers (22 bits of it; one alone, 11 bits, is 2.6e-4 off the formula in 64
 // bits where two are 1.9e-4, which is the result's own rounding), so that a unit of 32 keys by 32 queries, 128 dims, has 24 matrix
-// instructions, 768 cycles.  16384 tokens, 16 heads of 128, causal, fp16: 1.69 ms (1.24 with one number).  Of larger tiles and other
-// orders, with one number, 4096 tokens, 16 heads of 128: 32 keys a wave 159 us, 64 keys 166; through registers and turned there 172; the
-// next unit's first product in front of this one's exponentials 192 (its registers spill).  fp32, whose matrix instructions are a sixteenth as fast: 4096 tokens, 8
-// heads of 128, 685 us, 100 TFLOP/s (library: 154).
+// instructions, 768 cycles, and about 720 of vector ones.  By counters a SIMD's two waves take turns with them more than they overlap:
+// 16384 tokens, 16 heads of 128, causal, fp16 take 1.63 to 1.69 ms (1.24 with one number), of which the matrix unit is busy 50 %, the
+// vector unit 54 %, LDS 17 % (no conflicts), at 1.9 GHz.  Of larger tiles and other orders, with one number, 4096 tokens, 16 heads of 128:
+// 32 keys a wave 159 us, 64 keys 166; through registers and turned there 172; the next unit's first product in front of this one's
+// exponentials 192 (its registers spill).  fp32, whose matrix instructions are a sixteenth as fast: 4096 tokens, 8 heads of 128, 763 us,
+// 90 TFLOP/s (library: 154).
 #include "attention_common.h"
 
 namespace fynhip {

@@ -66,10 +66,11 @@ static int tiled(const AttnParams& p, int tokens) {
     if (p.dim > 128 && !p.f16) return 0;
     if (!p.paged && std::max(p.k.tok, p.v.tok) * (p.f16 ? 2 : 4) > (1 << 24)) return 0;      // (32 bits of offset within a tile)
     // Large workgroups read keys and values the fewest times, small ones are more: 128 queries where that gives two workgroups
-    // for each CU (32 heads, 4 ragged prompts of up to 2001 tokens, window 512, fp16: 115 us, against 134 with 64; half as many
-    // workgroups, 8 heads of 2048 tokens, two sequences: 58 us, against 39 with 64), 64 where it gives them for three quarters of the
-    // CUs (12 heads of 197 tokens, four sequences: 8.0 us, against 10.7 without tiles; 8 heads of 1024 tokens, fp32, which is half
-    // of the CUs: 99 us, against 64).
+    // for each CU (16 heads of 4096 tokens, both ways: 222 us, against 243 with 64; causal, with runs of unequal length, 153 against 138;
+    // half as many workgroups, 8 heads of 2048 tokens, two sequences: 71 us, against 49 with 64), 64 where it gives them for three quarters of
+    // the CUs (12 heads of 197 tokens, four sequences: 8.9 us, against 11.4 without tiles; 8 heads of 1024 tokens of 64 values, fp32, which is
+    // half of the CUs: 53 us, against 27).  Sequences count as long as the longest: of many short ones beside a long one most workgroups are
+    // empty or have few queries.
     const int64_t units = (int64_t)p.batch * p.heads;
     if (units * ((tokens + 127) / 128) >= 512) return 128;
     if (units * ((tokens + 63) / 64) >= 192) return 64;
