@@ -264,7 +264,8 @@ int fyn_net_set_buffer_reuse(fyn_net* net, int enable);
 int fyn_net_use_graph(fyn_net* net, int enable);
 
 /* Measurement helpers (no reference counterpart): time `iters` forwards between two hipEvents on the
- * network's stream; per-layer variant times one layer's kernels alone.  Milliseconds total. */
+ * network's stream; per-layer variant times one layer's kernels alone (of a layer that is bound to a cache: for the batch as it is then,
+ * whose keys and values it writes).  Milliseconds total. */
 int fyn_net_time_forward(fyn_net* net, int iters, float* ms_total);
 int fyn_layer_time(fyn_net* net, int layer, int iters, float* ms_total);
 /* `iters` forward passes queued back to back with an event after each; ms_each[i] receives the GPU time between the
